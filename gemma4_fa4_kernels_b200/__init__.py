@@ -27,6 +27,7 @@ from .model_spec import (
     AttentionLayerSpec,
     Gemma4ModelSpec,
 )
+from .paged_cache import PagedKVCache8
 from .prep import (
     prepare_global_kv_from_projection_source,
     prepare_rotary_operand,
@@ -61,6 +62,7 @@ __all__ = [
     "UnsupportedH100Path",
     "gemma4_attention_mask",
     "additive_mask",
+    "PagedKVCache8",
     "BACKEND_NAME",
     "Gemma4DispatchResult",
     "Gemma4MaskPlan",

@@ -48,6 +48,18 @@ EXPORTED_SYMBOLS = (
     "g4_prep_bwd_workspace_bytes",
     "g4_prep_fwd",
     "g4_prep_bwd",
+    "g4_kv8_append",
+    "g4_kv8_read",
+    "g4_kv8_attn_workspace_bytes",
+    "g4_kv8_attn",
+    "g4_kv8_chunk_plan",
+    "g4_kv8_pad_rows",
+    "g4_pages_workspace_bytes",
+    "g4_pages_extend",
+    "g4_pages_fork",
+    "g4_pages_free",
+    "g4_pages_compact",
+    "g4_pages_copy",
     "g4_kernel_count",
     "g4_kernel_name",
     "g4_launch_count",
@@ -155,6 +167,89 @@ class G4PrepArgs(ctypes.Structure):
     ]
 
 
+G4_KV8_E4M3 = 0
+G4_KV8_INT8 = 1
+
+
+class G4Kv8Args(ctypes.Structure):
+    """Mirror of ``g4_kv8_args``."""
+
+    _fields_ = [
+        ("k_pages", ctypes.c_void_p),
+        ("v_pages", ctypes.c_void_p),
+        ("k_scale", ctypes.c_void_p),
+        ("v_scale", ctypes.c_void_p),
+        ("tables", ctypes.c_void_p),
+        ("format", ctypes.c_int32),
+        ("num_pages", ctypes.c_int32),
+        ("page_size", ctypes.c_int32),
+        ("num_kv_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("num_slots", ctypes.c_int32),
+        ("pages_per_slot", ctypes.c_int32),
+        ("batch", ctypes.c_int32),
+        ("tokens", ctypes.c_int32),
+        ("slots", ctypes.c_void_p),
+        ("starts", ctypes.c_void_p),
+        ("ends", ctypes.c_void_p),
+        ("status", ctypes.c_void_p),
+        ("k", ctypes.c_void_p),
+        ("v", ctypes.c_void_p),
+        ("k_stride", ctypes.c_int64 * 3),
+        ("v_stride", ctypes.c_int64 * 3),
+        ("out_rows", ctypes.c_void_p),
+        ("out_total", ctypes.c_int32),
+        ("q", ctypes.c_void_p),
+        ("o", ctypes.c_void_p),
+        ("lse", ctypes.c_void_p),
+        ("q_stride", ctypes.c_int64 * 3),
+        ("o_stride", ctypes.c_int64 * 3),
+        ("lse_stride", ctypes.c_int64 * 2),
+        ("num_q_heads", ctypes.c_int32),
+        ("window", ctypes.c_int32),
+        ("max_seqlen_k", ctypes.c_int32),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
+# bits of a cache's status word
+G4_PAGES_EXHAUSTED = 1
+G4_PAGES_ROW_FULL = 2
+G4_PAGES_BAD_INDEX = 4
+
+
+class G4PagesArgs(ctypes.Structure):
+    """Mirror of ``g4_pages_args``."""
+
+    _fields_ = [
+        ("tables", ctypes.c_void_p),
+        ("lengths", ctypes.c_void_p),
+        ("refcounts", ctypes.c_void_p),
+        ("status", ctypes.c_void_p),
+        ("k_pages", ctypes.c_void_p),
+        ("v_pages", ctypes.c_void_p),
+        ("k_scale", ctypes.c_void_p),
+        ("v_scale", ctypes.c_void_p),
+        ("num_layers", ctypes.c_int32),
+        ("num_pages", ctypes.c_int32),
+        ("page_size", ctypes.c_int32),
+        ("num_kv_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32),
+        ("num_slots", ctypes.c_int32),
+        ("pages_per_slot", ctypes.c_int32),
+        ("batch", ctypes.c_int32),
+        ("first", ctypes.c_void_p),
+        ("second", ctypes.c_void_p),
+        ("counts", ctypes.c_void_p),
+        ("starts", ctypes.c_void_p),
+        ("ends", ctypes.c_void_p),
+        ("window", ctypes.c_int32),
+        ("workspace", ctypes.c_void_p),
+        ("workspace_bytes", ctypes.c_size_t),
+    ]
+
+
 _lock = threading.Lock()
 _lib: ctypes.CDLL | None = None
 
@@ -221,6 +316,23 @@ def load() -> ctypes.CDLL:
         for name in ("g4_prep_fwd", "g4_prep_bwd"):
             fn = getattr(lib, name)
             fn.argtypes = [PP, ctypes.c_void_p]
+            fn.restype = ctypes.c_int
+        K8 = ctypes.POINTER(G4Kv8Args)
+        for name in ("g4_kv8_append", "g4_kv8_read", "g4_kv8_attn", "g4_kv8_pad_rows"):
+            fn = getattr(lib, name)
+            fn.argtypes = [K8, ctypes.c_void_p]
+            fn.restype = ctypes.c_int
+        lib.g4_kv8_attn_workspace_bytes.argtypes = [K8]
+        lib.g4_kv8_attn_workspace_bytes.restype = ctypes.c_size_t
+        lib.g4_kv8_chunk_plan.argtypes = [K8] + [ctypes.c_void_p] * 5
+        lib.g4_kv8_chunk_plan.restype = ctypes.c_int
+        PG = ctypes.POINTER(G4PagesArgs)
+        lib.g4_pages_workspace_bytes.argtypes = [PG]
+        lib.g4_pages_workspace_bytes.restype = ctypes.c_size_t
+        for name in ("g4_pages_extend", "g4_pages_fork", "g4_pages_free", "g4_pages_compact",
+                     "g4_pages_copy"):
+            fn = getattr(lib, name)
+            fn.argtypes = [PG, ctypes.c_void_p]
             fn.restype = ctypes.c_int
         lib.g4_kernel_count.restype = ctypes.c_int
         lib.g4_kernel_name.argtypes = [ctypes.c_int]

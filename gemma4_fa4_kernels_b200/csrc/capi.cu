@@ -14,6 +14,7 @@
 #include <vector>
 
 #include "../../include/gemma4_b200.h"
+#include "g4_api.h"
 #include "g4_kernels.h"
 
 namespace {
@@ -38,33 +39,7 @@ int cuda_fail(cudaError_t e, const char* what) {
 // ---------------------------------------------------------------------------------------
 // launch accounting / opt-in event timing
 // ---------------------------------------------------------------------------------------
-enum KernelId {
-  kKFwd = 0,
-  kKBwdPre,
-  kKBwdDq,
-  kKBwdDkv,
-  kKPlan,
-  kKMask,
-  kKScore,
-  kKGemmDv,
-  kKGemmDk,
-  kKGemmDq,
-  kKFwdScore,
-  kKFwdPv,
-  kKDecode,
-  kKDecodeCombine,
-  kKPrepFwd,
-  kKPrepBwd,
-  kKPrepDw,
-  kKSelftest,
-  kKGemmDvDk,
-  kKCast,
-  kKMerge,
-  kKAdd,
-  kKDecodeShort,
-  kKReset,
-  kKCount
-};
+using namespace g4;  // KernelId, LaunchScope (g4_api.h)
 const char* const kKernelNames[kKCount] = {"attn_fwd", "bwd_preprocess", "bwd_dq", "bwd_dkv",
                                            "plan",     "mask",           "bwd_score",
                                            "bwd_gemm_dv", "bwd_gemm_dk", "bwd_gemm_dq",
@@ -72,7 +47,9 @@ const char* const kKernelNames[kKCount] = {"attn_fwd", "bwd_preprocess", "bwd_dq
                                            "decode_combine", "prep_fwd",  "prep_bwd",
                                            "prep_dw_reduce", "selftest_wait", "bwd_gemm_dvdk",
                                            "cast_f32_bf16", "ring_merge", "add_f32",
-                                           "decode_short", "workspace_reset"};
+                                           "decode_short", "workspace_reset", "kv8_attn",
+                                           "kv8_merge",   "kv8_append", "kv8_read",
+                                           "kv8_chunk",   "pages_plan", "pages_apply"};
 std::atomic<long long> g_launches[kKCount];
 std::atomic<bool> g_profile{false};
 struct ProfRecord {
@@ -81,32 +58,6 @@ struct ProfRecord {
 };
 std::mutex g_prof_mu;
 std::vector<ProfRecord> g_prof_records;
-
-// Brackets one launch: counts it and, when profiling, records events around it.
-class LaunchScope {
- public:
-  LaunchScope(int id, cudaStream_t st) : id_(id), st_(st) {
-    g_launches[id].fetch_add(1);
-    if (g_profile.load()) {
-      if (cudaEventCreate(&a_) == cudaSuccess && cudaEventCreate(&b_) == cudaSuccess) {
-        cudaEventRecord(a_, st_);
-        timed_ = true;
-      }
-    }
-  }
-  ~LaunchScope() {
-    if (!timed_) return;
-    cudaEventRecord(b_, st_);
-    std::lock_guard<std::mutex> lk(g_prof_mu);
-    g_prof_records.push_back({id_, a_, b_});
-  }
-
- private:
-  int id_;
-  cudaStream_t st_;
-  cudaEvent_t a_{}, b_{};
-  bool timed_ = false;
-};
 
 // ---------------------------------------------------------------------------------------
 // TMA tensor maps (driver entry point fetched through the runtime, no -lcuda needed)
@@ -1020,6 +971,39 @@ int noalloc_scratch(void** out) {
 }
 
 }  // namespace
+
+namespace g4 {
+
+LaunchScope::LaunchScope(int id, cudaStream_t st) : id_(id), st_(st) {
+  g_launches[id].fetch_add(1);
+  if (g_profile.load()) {
+    if (cudaEventCreate(&a_) == cudaSuccess && cudaEventCreate(&b_) == cudaSuccess) {
+      cudaEventRecord(a_, st_);
+      timed_ = true;
+    }
+  }
+}
+LaunchScope::~LaunchScope() {
+  if (!timed_) return;
+  cudaEventRecord(b_, st_);
+  std::lock_guard<std::mutex> lk(g_prof_mu);
+  g_prof_records.push_back({id_, a_, b_});
+}
+
+int api_fail(int code, const char* fmt, ...) {
+  char buf[512];
+  va_list ap;
+  va_start(ap, fmt);
+  vsnprintf(buf, sizeof(buf), fmt, ap);
+  va_end(ap);
+  g_last_error = buf;
+  return code;
+}
+int api_cuda_fail(cudaError_t e, const char* what) { return cuda_fail(e, what); }
+void api_clear_error() { g_last_error.clear(); }
+int api_sm_count() { return sm_count(); }
+
+}  // namespace g4
 
 extern "C" {
 

@@ -1,0 +1,199 @@
+// The 8-bit paged KV cache shared by its kernels (kv8_attn.cu, kv8_store.cu):
+// device view of one layer, rows of a call, and the codes' conversions.
+//
+// Keys and values of one layer live in pages of `page` tokens, each page
+// [kv head][token][head_dim] codes of 8 bits (e4m3 or int8); a block is one page
+// of one head and has one fp32 scale, value = code * scale.  The append writes
+// scales that are powers of two: a block whose scale has to grow when later
+// tokens join it then shifts its older codes exactly (up to the codes that fall
+// below the smallest step), quantising is an exact multiplication and one
+// rounding, and e4m3 codes lose nothing to the coarser choice (their relative
+// step does not depend on the scale).
+//
+// A table row lists the pages of one sequence in order, -1 where there is none.
+// Rows, page ids and positions that the device arrays carry are checked where
+// they are used: an out-of-range page is never read or written (its keys count
+// as masked), and a row whose slot or positions are out of range counts as empty.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace g4 {
+
+constexpr int kKv8MaxBatch = 1024;  // rows of one call (their plan sits in shared memory)
+constexpr int kKv8Tile = 16;        // keys per tile; page sizes are multiples of it
+constexpr int kKv8Cols = 8;         // (token, query head) columns of one attention item
+constexpr int kKv8Warps = 8;        // warps per attention CTA
+// exponents of a block's scale 2^e: 2^e and 2^-e are both normal fp32 values, and
+// the largest finite bf16 value fits 448 * 2^120 and 127 * 2^122
+constexpr int kKv8MinExp = -100;
+constexpr int kKv8MaxExp = 122;
+
+struct Kv8Cache {
+  uint8_t* k;               // [page][head][token][head_dim]
+  uint8_t* v;
+  float* k_scale;           // [page][head]
+  float* v_scale;
+  const int* tables;        // [slot][pages_per_slot]
+  int num_pages;
+  int page;                 // tokens per page: 16, 32, 64 or 128
+  int page_shift;
+  int heads;
+  int num_slots;
+  int pages_per_slot;
+};
+
+struct Kv8Rows {
+  const int* slots;         // nullable: row b uses slot b
+  const int* starts;        // position of the row's first token
+  const int* ends;          // one past its last
+  int batch;
+  int tokens;               // tokens (queries) per row in the operand; a row uses the first
+                            // min(end - start, tokens), the rest is padding
+};
+
+struct Kv8Row {
+  int slot;                 // -1: empty row
+  int start;
+  int n;                    // tokens of the row, <= rows.tokens
+};
+
+// Checked row b: empty (slot -1, n 0) when its slot or positions are out of range.
+__device__ __forceinline__ Kv8Row kv8_row(const Kv8Cache& c, const Kv8Rows& r, int b, int max_end) {
+  Kv8Row o;
+  const int slot = r.slots ? r.slots[b] : b;
+  const int start = r.starts[b], end = r.ends[b];
+  const bool ok = slot >= 0 && slot < c.num_slots && start >= 0 && end > start && end <= max_end &&
+                  (end - 1) >> c.page_shift < c.pages_per_slot;
+  o.slot = ok ? slot : -1;
+  o.start = ok ? start : 0;
+  o.n = ok ? min(end - start, r.tokens) : 0;
+  return o;
+}
+
+// Page of a position; -1 when there is none.
+__device__ __forceinline__ int kv8_page(const Kv8Cache& c, int slot, int pos) {
+  const int id = c.tables[static_cast<int64_t>(slot) * c.pages_per_slot + (pos >> c.page_shift)];
+  return id >= 0 && id < c.num_pages ? id : -1;
+}
+
+// Four codes (one word, byte i = element i) to fp16 pairs (0, 1) and (2, 3).  Both
+// formats fit fp16 exactly (e4m3: 4 significant bits from 2^-9 to 448; int8: 7).
+template <bool kInt8>
+__device__ __forceinline__ void kv8_to_half(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  if constexpr (kInt8) {
+    // byte b + 128 in the low mantissa bits of 1024 gives 1024 + 128 + b
+    const uint32_t x = w ^ 0x80808080u;
+    const __half2 off = __half2half2(__ushort_as_half(0x6480));  // 1152
+    const uint32_t a = __byte_perm(x, 0x64646464u, 0x4140);
+    const uint32_t b = __byte_perm(x, 0x64646464u, 0x4342);
+    const __half2 ha = __hsub2(*reinterpret_cast<const __half2*>(&a), off);
+    const __half2 hb = __hsub2(*reinterpret_cast<const __half2*>(&b), off);
+    lo = *reinterpret_cast<const uint32_t*>(&ha);
+    hi = *reinterpret_cast<const uint32_t*>(&hb);
+  } else {
+    asm("{\n\t.reg .b16 l, h;\n\t"
+        "mov.b32 {l, h}, %2;\n\t"
+        "cvt.rn.f16x2.e4m3x2 %0, l;\n\t"
+        "cvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+        : "=r"(lo), "=r"(hi)
+        : "r"(w));
+  }
+}
+
+// ---- attention (kv8_attn.cu) ----
+struct Kv8AttnParams {
+  Kv8Cache cache;
+  Kv8Rows rows;
+  int window;               // 0: every earlier key
+  int max_k;                // rows that end past it count as empty
+  int group;                // query heads per KV head
+  int col_blocks;           // ceil(tokens * group / kKv8Cols)
+  const __nv_bfloat16* q;   // (batch, token, head) strides in elements
+  int64_t q_stride[3];
+  __nv_bfloat16* o;
+  int64_t o_stride[3];
+  float* lse;               // (batch, head) strides; token stride 1
+  int64_t lse_stride[2];
+  // partial results (workspace): two per warp, [warp][head, tail]
+  float* part_o;            // [slot][head_dim * kKv8Cols] in fragment order
+  float4* part_ml;          // [slot][kKv8Cols]: (shift of O, max, sum, -)
+  int* plan;                // [0] tiles per warp, [1..batch+1] first tile of each row
+};
+int launch_kv8_attn(int d, bool int8, const Kv8AttnParams& p, int ctas, cudaStream_t stream);
+int launch_kv8_merge(int d, const Kv8AttnParams& p, cudaStream_t stream);
+
+// ---- append, read back, chunks of prompts (kv8_store.cu) ----
+struct Kv8StoreParams {
+  Kv8Cache cache;
+  Kv8Rows rows;
+  const __nv_bfloat16* k;   // append: (batch, token, head) strides in elements
+  const __nv_bfloat16* v;
+  int64_t k_stride[3];
+  int64_t v_stride[3];
+  __nv_bfloat16* k_out;     // read: same strides for both
+  __nv_bfloat16* v_out;
+  int64_t out_stride[3];
+  const int* out_rows;      // read, nullable: rows packed, row b at [out_rows[b], out_rows[b+1])
+  int out_total;            // packed: rows of the output
+  int* status;              // nullable
+};
+int launch_kv8_append(int d, bool int8, const Kv8StoreParams& p, cudaStream_t stream);
+int launch_kv8_read(int d, bool int8, const Kv8StoreParams& p, cudaStream_t stream);
+
+struct Kv8ChunkParams {
+  Kv8Cache cache;
+  Kv8Rows rows;
+  int window;
+  int max_k;
+  int* cu_q;                // [batch + 1]
+  int* cu_k;                // [batch + 1]
+  int* first;               // [batch] first key read
+  int* last;                // [batch] one past the last key read
+};
+int launch_kv8_chunk_plan(const Kv8ChunkParams& p, cudaStream_t stream);
+// zeros (LSE: -inf) in the rows of a chunk's output that are padding
+int launch_kv8_pad_rows(const Kv8Cache& c, const Kv8Rows& r, int max_k, int heads, int d,
+                        __nv_bfloat16* o, const int64_t* o_stride, float* lse,
+                        const int64_t* lse_stride, cudaStream_t stream);
+
+// ---- pages (kv8_pages.cu) ----
+enum Kv8Status : int {
+  kKv8PoolExhausted = 1,    // no free page left for a row
+  kKv8RowFull = 2,          // a row's table is full
+  kKv8BadIndex = 4,         // slot, page or count out of range, or the same one twice
+};
+struct Kv8PagesParams {
+  int* tables;
+  int* lengths;
+  int* refcounts;
+  int* status;
+  int num_pages, page, page_shift, num_slots, pages_per_slot;
+  // the pools of all layers, as bytes
+  uint8_t* k;
+  uint8_t* v;
+  float* k_scale;
+  float* v_scale;
+  int layers, heads;
+  int64_t page_bytes;       // heads * page * head_dim
+  const int* a;             // slots, parents or source pages
+  const int* b;             // children or destination pages
+  const int* counts;
+  int* starts;
+  int* ends;
+  int batch;
+  int window;               // free: 0 everything, > 0 only what a window no longer reaches
+  int* work;                // workspace
+};
+int launch_pages_extend(const Kv8PagesParams& p, cudaStream_t stream);
+int launch_pages_fork_plan(const Kv8PagesParams& p, cudaStream_t stream);
+int launch_pages_fork_apply(const Kv8PagesParams& p, int ctas, cudaStream_t stream);
+int launch_pages_free(const Kv8PagesParams& p, cudaStream_t stream);
+int launch_pages_compact_plan(const Kv8PagesParams& p, cudaStream_t stream);
+int launch_pages_compact_apply(const Kv8PagesParams& p, int ctas, cudaStream_t stream);
+int launch_pages_copy(const Kv8PagesParams& p, int ctas, cudaStream_t stream);
+
+}  // namespace g4

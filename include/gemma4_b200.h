@@ -329,6 +329,155 @@ int g4_prep_fwd(const g4_prep_args* args, void* stream);
 int g4_prep_bwd(const g4_prep_args* args, void* stream);
 
 /*
+ * 8-bit paged KV cache (no reference counterpart: the reference's static caches
+ * are bf16 and contiguous, h100_torch_ops.py:692-880).
+ *
+ * Keys and values of one layer live in pages of `page_size` tokens, each page
+ * [kv head][token][head_dim] codes of 8 bits (G4_KV8_E4M3 or G4_KV8_INT8).  A
+ * block is one page of one KV head; it has one fp32 scale in k_scale / v_scale
+ * [page][kv head], and its values are code * scale.  Codes are finite and scales
+ * positive and finite; g4_kv8_append writes powers of two.  tables
+ * [slot][pages_per_slot] lists a sequence's pages in order (-1: none).
+ *
+ * A call serves `batch` rows.  Row b uses table row slots[b] (b itself when slots
+ * is null), its tokens sit at positions starts[b] .. ends[b] - 1, and they are the
+ * first min(ends[b] - starts[b], tokens) of its `tokens` rows in the operands; the
+ * rest is padding.  A row with ends[b] <= starts[b], or whose slot or positions
+ * are out of range, is empty.  These arrays are read on the device.  At most 1024
+ * rows; page sizes 16, 32, 64 and 128; head dims 256 and 512; operand strides in
+ * elements, multiples of 8; 16-byte aligned bases.
+ */
+enum g4_kv8_format { G4_KV8_E4M3 = 0, G4_KV8_INT8 = 1 };
+typedef struct g4_kv8_args {
+  /* one layer of the cache */
+  void* k_pages;
+  void* v_pages;
+  float* k_scale;
+  float* v_scale;
+  const int32_t* tables;
+  int32_t format;
+  int32_t num_pages;
+  int32_t page_size;
+  int32_t num_kv_heads;
+  int32_t head_dim;
+  int32_t num_slots;
+  int32_t pages_per_slot;
+  /* rows */
+  int32_t batch;
+  int32_t tokens;
+  const int32_t* slots; /* nullable */
+  const int32_t* starts;
+  const int32_t* ends;
+  int32_t* status;      /* append, nullable: device word, G4_PAGES_* bits are or-ed in */
+  /* append: inputs; read: outputs; [batch][token][kv head][head_dim] bf16 */
+  void* k;
+  void* v;
+  int64_t k_stride[3]; /* batch, token, head */
+  int64_t v_stride[3];
+  const int32_t* out_rows; /* read, nullable: packed output, row b fills [out_rows[b],
+                              out_rows[b + 1]) (at most `tokens` rows); batch strides unused */
+  int32_t out_total;       /* packed: rows of the outputs; up to 128 behind the last segment
+                              are zeroed */
+  /* attention */
+  const void* q; /* [batch][token][query head][head_dim] bf16 */
+  void* o;
+  float* lse;    /* token stride 1 */
+  int64_t q_stride[3];
+  int64_t o_stride[3];
+  int64_t lse_stride[2]; /* batch, head */
+  int32_t num_q_heads;
+  int32_t window;       /* 0: every earlier key; W > 0: keys k > position - W */
+  int32_t max_seqlen_k; /* upper bound of ends; a row beyond it is empty */
+  void* workspace;
+  size_t workspace_bytes;
+} g4_kv8_args;
+
+/*
+ * Quantise the rows' K and V and write them at their positions.  A block's scale
+ * is the least power of two 2^e with max|x| <= 448 * 2^e (e4m3) or 127 * 2^e
+ * (int8) over its finite values; when tokens join a page that holds earlier ones
+ * it only grows, and the earlier codes are requantised.  Infinities saturate, NaN
+ * becomes 0.  Slots must be distinct: a slot listed again is left out (status).
+ */
+int g4_kv8_append(const g4_kv8_args* args, void* stream);
+/* K and V of the rows' positions as bf16; zeros past a row's end and where the
+ * table has no page. */
+int g4_kv8_read(const g4_kv8_args* args, void* stream);
+/*
+ * Attention of the rows' queries (softmax scale 1) over the keys 0 .. position of
+ * their own sequence, cut by the window; the keys of missing pages are masked.
+ * A query without a visible key, and padding, gets O = 0 and LSE = -inf.  Meant
+ * for a few queries per row; g4_kv8_chunk_plan serves prompt chunks.
+ */
+size_t g4_kv8_attn_workspace_bytes(const g4_kv8_args* args);
+int g4_kv8_attn(const g4_kv8_args* args, void* stream);
+/*
+ * Prompt chunks: g4_kv8_chunk_plan writes the segments of g4_attn_fwd's packed
+ * layout (cu_q, cu_k: batch + 1 entries; row b's queries are its `tokens` rows,
+ * its keys the positions [first[b], starts[b] + tokens)) and the positions
+ * [first[b], last[b]) to read back into them (g4_kv8_read with starts = first,
+ * ends = last, out_rows = cu_k); g4_kv8_pad_rows then clears the outputs of
+ * padding and of empty rows.
+ */
+int g4_kv8_chunk_plan(const g4_kv8_args* args, int32_t* cu_q, int32_t* cu_k, int32_t* first,
+                      int32_t* last, void* stream);
+int g4_kv8_pad_rows(const g4_kv8_args* args, void* stream);
+
+/*
+ * Pages of such a cache, all layers at once; the state lives on the device and no
+ * call reads it back.  lengths[slot]: tokens; refcounts[page]: tables that list
+ * the page (0 = free).  Pages are taken from the lowest free ids in order of the
+ * rows.  A row that cannot be served is left as it was and raises a bit of *status:
+ * G4_PAGES_EXHAUSTED no free page (rows are served in order until the pool is
+ * empty), G4_PAGES_ROW_FULL its table is full, G4_PAGES_BAD_INDEX an index out of
+ * range or listed twice.
+ */
+#define G4_PAGES_EXHAUSTED 1
+#define G4_PAGES_ROW_FULL 2
+#define G4_PAGES_BAD_INDEX 4
+typedef struct g4_pages_args {
+  int32_t* tables;
+  int32_t* lengths;
+  int32_t* refcounts;
+  int32_t* status;
+  void* k_pages;  /* [layer][page] pools */
+  void* v_pages;
+  float* k_scale; /* [layer][page][kv head] */
+  float* v_scale;
+  int32_t num_layers;
+  int32_t num_pages;
+  int32_t page_size;
+  int32_t num_kv_heads;
+  int32_t head_dim;
+  int32_t num_slots;
+  int32_t pages_per_slot;
+  int32_t batch;         /* rows of this call, at most 1024 (copy: any number) */
+  const int32_t* first;  /* extend, free: slots; fork: parents; copy: source pages */
+  const int32_t* second; /* fork: children; copy: destination pages */
+  const int32_t* counts; /* extend: new tokens */
+  int32_t* starts;       /* extend, out: position of the row's first new token */
+  int32_t* ends;         /* extend, out: one past its last (= start: not served) */
+  int32_t window;        /* free: 0 frees the rows; W > 0 only the leading pages that no
+                            token from position `length` on sees through the window */
+  void* workspace;
+  size_t workspace_bytes;
+} g4_pages_args;
+
+size_t g4_pages_workspace_bytes(const g4_pages_args* args);
+/* Reserve pages for counts[b] more tokens of each slot and advance its length. */
+int g4_pages_extend(const g4_pages_args* args, void* stream);
+/* Make each child (an empty slot) a copy of its parent: whole pages are shared, a
+ * partly filled last page is copied. */
+int g4_pages_fork(const g4_pages_args* args, void* stream);
+int g4_pages_free(const g4_pages_args* args, void* stream);
+/* Move the live pages to the lowest ids: each page at or above the number of live
+ * pages goes to a hole below it, both in ascending order. */
+int g4_pages_compact(const g4_pages_args* args, void* stream);
+/* Copy pages; tables and refcounts stay.  A pair whose destination an earlier pair
+ * has too, or is any pair's source, is left out (status). */
+int g4_pages_copy(const g4_pages_args* args, void* stream);
+
+/*
  * Launch accounting and opt-in timing (benchmark/profiling support; no
  * reference counterpart -- the reference times whole Python calls).
  * Kernel ids: 0 forward, 1 backward preprocess, 2 backward dQ (recompute),
@@ -341,7 +490,10 @@ int g4_prep_bwd(const g4_prep_args* args, void* stream);
  * the dO and Q operands take at most 80 MiB together), 19 fp32 -> bf16 cast
  * (the dV / dK of a multi-band backward), 20 ring merge of a partial output,
  * 21 fp32 add (halo key gradients), 22 short-window decode (sliding layers,
- * query groups of at most 4 heads: one launch, merge fused).
+ * query groups of at most 4 heads: one launch, merge fused), 23 workspace reset,
+ * 24 attention over the 8-bit paged cache, 25 the sum of its parts, 26 append,
+ * 27 read back, 28 chunk plan and padding, 29 page planning (extend, fork, free,
+ * compact), 30 page copies and table updates.
  *  - g4_launch_count: launches of `kernel_id` issued by this process so far.
  *  - g4_profile_enable(1): every later launch is bracketed by CUDA events on
  *    its own stream; g4_profile_read synchronises those events and returns the
