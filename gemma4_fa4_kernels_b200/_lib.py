@@ -208,6 +208,7 @@ class G4Kv8Args(ctypes.Structure):
         ("num_q_heads", ctypes.c_int32),
         ("window", ctypes.c_int32),
         ("max_seqlen_k", ctypes.c_int32),
+        ("device", ctypes.c_int32),
         ("workspace", ctypes.c_void_p),
         ("workspace_bytes", ctypes.c_size_t),
     ]
@@ -245,6 +246,7 @@ class G4PagesArgs(ctypes.Structure):
         ("starts", ctypes.c_void_p),
         ("ends", ctypes.c_void_p),
         ("window", ctypes.c_int32),
+        ("device", ctypes.c_int32),
         ("workspace", ctypes.c_void_p),
         ("workspace_bytes", ctypes.c_size_t),
     ]

@@ -24,13 +24,17 @@
 namespace g4 {
 
 constexpr int kKv8MaxBatch = 1024;  // rows of one call (their plan sits in shared memory)
-constexpr int kKv8Tile = 16;        // keys per tile; page sizes are multiples of it
-constexpr int kKv8Cols = 8;         // (token, query head) columns of one attention item
-constexpr int kKv8Warps = 8;        // warps per attention CTA
+constexpr int kKv8Tile = 32;        // keys per attention tile: two pieces of 16, each in one page
 // exponents of a block's scale 2^e: 2^e and 2^-e are both normal fp32 values, and
 // the largest finite bf16 value fits 448 * 2^120 and 127 * 2^122
 constexpr int kKv8MinExp = -100;
 constexpr int kKv8MaxExp = 122;
+
+enum Kv8Status : int {
+  kKv8PoolExhausted = 1,    // no free page left for a row
+  kKv8RowFull = 2,          // a row's table is full
+  kKv8BadIndex = 4,         // slot, page or count out of range, or the same one twice
+};
 
 struct Kv8Cache {
   uint8_t* k;               // [page][head][token][head_dim]
@@ -111,20 +115,28 @@ struct Kv8AttnParams {
   int window;               // 0: every earlier key
   int max_k;                // rows that end past it count as empty
   int group;                // query heads per KV head
-  int col_blocks;           // ceil(tokens * group / kKv8Cols)
+  int cols;                 // (token, query head) columns of one item (Kv8AttnShape)
+  int col_groups;           // ceil(tokens * group / cols)
   const __nv_bfloat16* q;   // (batch, token, head) strides in elements
   int64_t q_stride[3];
   __nv_bfloat16* o;
   int64_t o_stride[3];
   float* lse;               // (batch, head) strides; token stride 1
   int64_t lse_stride[2];
-  // partial results (workspace): two per warp, [warp][head, tail]
-  float* part_o;            // [slot][head_dim * kKv8Cols] in fragment order
-  float4* part_ml;          // [slot][kKv8Cols]: (shift of O, max, sum, -)
-  int* plan;                // [0] tiles per warp, [1..batch+1] first tile of each row
+  // partial results (workspace): two per run, [run][head, tail]
+  float* part_o;            // [slot][cols][head_dim]
+  float4* part_ml;          // [slot][cols]: (shift of O, max, sum, -)
+  int* plan;                // {runs, tiles, -, -}, the rows' plans (int4 each), their first tiles
 };
+// The kernel's launch shape for a row's number of (token, query head) columns.
+struct Kv8AttnShape {
+  int cols;                 // columns one pass over the codes serves
+  int runs;                 // runs per CTA
+  int out_floats;           // floats of a partial O
+};
+Kv8AttnShape kv8_attn_shape(int d, int64_t columns);
 int launch_kv8_attn(int d, bool int8, const Kv8AttnParams& p, int ctas, cudaStream_t stream);
-int launch_kv8_merge(int d, const Kv8AttnParams& p, cudaStream_t stream);
+int launch_kv8_merge(int d, const Kv8AttnParams& p, int ctas, cudaStream_t stream);
 
 // ---- append, read back, chunks of prompts (kv8_store.cu) ----
 struct Kv8StoreParams {
@@ -161,11 +173,6 @@ int launch_kv8_pad_rows(const Kv8Cache& c, const Kv8Rows& r, int max_k, int head
                         const int64_t* lse_stride, cudaStream_t stream);
 
 // ---- pages (kv8_pages.cu) ----
-enum Kv8Status : int {
-  kKv8PoolExhausted = 1,    // no free page left for a row
-  kKv8RowFull = 2,          // a row's table is full
-  kKv8BadIndex = 4,         // slot, page or count out of range, or the same one twice
-};
 struct Kv8PagesParams {
   int* tables;
   int* lengths;

@@ -16,13 +16,15 @@
 // shared memory, which a tcgen05 operand would need (3 times the shared-memory
 // traffic per byte read for 8 of at least 16 useful columns).
 //
-// Work split: every (sequence, KV head, column block) is an item of n 16-key
-// tiles; all items' tiles form one list, cut into equal runs, one per warp, so
-// ragged batches load every SM alike whatever the lengths are.  A warp streams its
-// run's K and V tiles through its own ring of padded shared-memory buffers
-// (cp.async), with no barrier against other warps.  An item that lies in one run
-// is written at once; the ends of the CTA's runs that belong to one item are
-// summed in shared memory; what then still spans CTAs goes to the workspace and
+// Work split: every (sequence, KV head, column group) is an item of n 32-key
+// tiles; all items' tiles form one list, cut into equal runs, one per team, so
+// ragged batches load every SM alike whatever the lengths are.  A team is kTeam
+// warps that hold kDims = D / kTeam dims each, of Q, K, V and O: their partial S
+// meet in shared memory (one named barrier per tile), everything else of a warp is
+// its own: it streams its dims of the run's K and V through its own ring of padded
+// shared-memory buffers (cp.async, 16 keys each).  An item that lies in one run is
+// written at once; the ends of the CTA's runs that belong to one item are summed
+// in shared memory; what then still spans CTAs goes to the workspace and
 // kv8_merge_kernel adds it up (in a fixed order: results do not depend on timing).
 //
 // Fragments: the dims of a K chunk and the dims and keys of a V chunk may be dealt
@@ -40,6 +42,8 @@
 // 2^11: below 2^15, rounded by at most 2^-12 of itself, or, for weights more than
 // 2^25 below the largest, by 2^-36 of the largest.  The output's rounding to bf16
 // is 2^-9 of it.
+#include <algorithm>
+
 #include "g4_kernels.h"
 #include "g4_sm100.cuh"
 #include "kv8.h"
@@ -51,27 +55,41 @@ namespace {
 constexpr float kShiftUp = 11.f;    // log2 of the factor on P
 constexpr float kStale = 3.f;       // log2 by which O's maximum may lag before a rescale
 
-template <int D>
-struct AttnCfg {
-  static constexpr int kRow = D + 16;                  // bytes per key row in a buffer
-  static constexpr int kBuf = kKv8Tile * kRow;
-  static constexpr int kBufs = D == 512 ? 3 : 6;       // K and V tiles in flight per warp
+// One launch shape: kTeam warps share a run, kBlocks blocks of 8 columns are
+// served by one pass over the codes.
+template <int kD, int kTeam_, int kBlocks_, int kWarps_, int kBufs_>
+struct AttnShape {
+  static constexpr int D = kD, kTeam = kTeam_, kBlocks = kBlocks_, kWarps = kWarps_;
+  static constexpr int kTeams = kWarps / kTeam;        // runs per CTA
+  static constexpr int kThreads = kWarps * 32;
+  static constexpr int kCols = 8 * kBlocks;
+  static constexpr int kDims = D / kTeam;              // dims per warp
+  static constexpr int kRow = kDims + 16;              // bytes per key row in a buffer
+  static constexpr int kBuf = 16 * kRow;
+  static constexpr int kBufs = kBufs_;                 // 16-key K or V pieces in flight per warp
   static constexpr int kRing = kBufs * kBuf;
-  static constexpr int kChunks = D / 64;               // K chunks per thread and row
-  static constexpr int kSteps = D / 128;               // V chunks per thread and key
-  static constexpr int kAcc = D / 4;                   // O registers per thread
-  static constexpr int kRingBytes = kKv8Warps * kRing;
-  static constexpr int kStatBytes = kKv8Warps * kKv8Cols * 16 + kKv8Warps * 4 * 4;
+  static constexpr int kChunks = kDims / 64;           // K chunks per thread and row
+  static constexpr int kSteps = kDims / 128;           // V chunks per thread and key
+  static constexpr int kTilesM = kDims / 16;           // MMAs over a warp's dims
+  static constexpr int kOut = D * kCols;               // floats of a partial O
+  static constexpr int kOutRow = D + 4;                // and of its columns in shared memory
+  static constexpr int kRingBytes = kWarps * kRing;
+  static constexpr int kSwaps = kTeam > 1 ? 2 : 1;     // copies of the S buffers
+  static constexpr int kExchange = kWarps * kSwaps * kBlocks * 1024;
+  static constexpr int kStats = kTeams * kCols * 16;
+  static constexpr int kTails = kTeams * 4 * 4;
+  static_assert(kRingBytes >= kTeams * kCols * kOutRow * 4, "the runs' ends are summed in the ring's place");
   static constexpr int smem(int batch) {
-    return kRingBytes + kStatBytes + 16 * batch + 4 * (batch + 1) + 64;
+    return kRingBytes + kExchange + kStats + ((kTails + 15) & ~15) + 16 * batch + 4 * (batch + 1) +
+           4 * kWarps;
   }
 };
 
-// A tile range's place: row, item within the row, tile.
+// A tile's place: row, item within the row, tile.
 struct Place {
   int b;
-  int item;     // active items (queries present) first, then the padded column blocks
-  int tile;     // absolute tile index (16 keys)
+  int item;     // active items (queries present) first, then the padded column groups
+  int tile;     // absolute tile index (32 keys)
   int left;     // tiles left in the item
 };
 
@@ -82,11 +100,29 @@ struct RowPlan {  // shared memory, one per row
   int lo;       // first visible key of the row
 };
 
-__device__ __forceinline__ int active_blocks(const RowPlan& r, int group) {
-  return (r.n * group + kKv8Cols - 1) / kKv8Cols;
+template <int kCols>
+__device__ __forceinline__ int active_groups(const RowPlan& r, int group) {
+  return (r.n * group + kCols - 1) / kCols;
 }
 __device__ __forceinline__ int row_tiles(const RowPlan& r) {
   return r.n > 0 ? (r.start + r.n + kKv8Tile - 1) / kKv8Tile - r.lo / kKv8Tile : 1;
+}
+__device__ __forceinline__ RowPlan row_plan(const Kv8AttnParams& p, int b) {
+  const Kv8Row r = kv8_row(p.cache, p.rows, b, p.max_k);
+  RowPlan rp;
+  rp.slot = r.slot;
+  rp.start = r.start;
+  rp.n = r.n;
+  rp.lo = p.window > 0 ? max(0, r.start - p.window + 1) : 0;
+  return rp;
+}
+
+// Run i of n over `total` tiles begins at floor(i * total / n); n <= total.
+__device__ __forceinline__ int run_begin(int i, int n, int total) {
+  return static_cast<int>(static_cast<int64_t>(i) * total / n);
+}
+__device__ __forceinline__ int run_of(int tile, int n, int total) {
+  return static_cast<int>((static_cast<int64_t>(tile + 1) * n - 1) / total);
 }
 
 __device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
@@ -98,60 +134,116 @@ __device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4],
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// 16 bytes global -> shared, zeros where `bytes` is 0.
-__device__ __forceinline__ void cp16(uint32_t dst, const void* src, int bytes) {
+// 16 (4) bytes global -> shared; the _z form writes zeros where `bytes` is 0.
+__device__ __forceinline__ void cp16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp16_z(uint32_t dst, const void* src, int bytes) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes)
                : "memory");
 }
-__device__ __forceinline__ void cp4(uint32_t dst, const void* src, int bytes) {
+__device__ __forceinline__ void cp4_z(uint32_t dst, const void* src, int bytes) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(src), "r"(bytes)
                : "memory");
 }
 
-// 2^(e) * value scaled exactly: the factor of a column's Q and its exponent.
+// Exponent of the power of two that brings a column's Q to [2^13, 2^14); zeros and
+// non-finite values stay.
 __device__ __forceinline__ int q_exponent(float amax) {
-  // amax in [2^(x-1), 2^x): bring it to [2^13, 2^14); zeros and non-finite values stay
   const int bits = static_cast<int>(__float_as_uint(amax) >> 23);
   if (bits == 0 || bits == 255) return 0;
   return min(13 - (bits - 127), 100);
 }
 
-// The 16 output dims of V chunk step i in thread row g: one 16-byte chunk.
+// 16-byte chunk of a V row (of the warp's dims) that thread row g takes in step i.
 __device__ __forceinline__ int v_chunk(int g, int i) { return (g & 1) * 4 + (g >> 1) + 8 * i; }
+
+// Factor from a held O (sum * 2^(kShiftUp - m_shift)) to the output; 0 without a key.
+__device__ __forceinline__ float out_factor(float m_shift, float m, float l) {
+  return l == 0.f || m_shift == -INFINITY ? 0.f : ex2(m_shift - kShiftUp - m) / l;
+}
+
+// Where column `col` of KV head `h` in row b goes: 16 consecutive dims, and its LSE.
+__device__ __forceinline__ void put_out(const Kv8AttnParams& p, int b, int h, int col, int dim,
+                                        const float (&v)[16], float f) {
+  const int tok = col / p.group;
+  if (tok >= p.rows.tokens) return;
+  uint32_t w[8];
+#pragma unroll
+  for (int x = 0; x < 8; ++x) w[x] = pack_bf16x2(v[2 * x] * f, v[2 * x + 1] * f);
+  uint4* dst = reinterpret_cast<uint4*>(
+      p.o + static_cast<int64_t>(b) * p.o_stride[0] + static_cast<int64_t>(tok) * p.o_stride[1] +
+      static_cast<int64_t>(h * p.group + col - tok * p.group) * p.o_stride[2] + dim);
+  dst[0] = make_uint4(w[0], w[1], w[2], w[3]);
+  dst[1] = make_uint4(w[4], w[5], w[6], w[7]);
+}
+// The same for four dims.
+__device__ __forceinline__ void put_dims(const Kv8AttnParams& p, int b, int h, int col, int dim,
+                                         const float4& v, float f) {
+  const int tok = col / p.group;
+  *reinterpret_cast<uint2*>(
+      p.o + static_cast<int64_t>(b) * p.o_stride[0] + static_cast<int64_t>(tok) * p.o_stride[1] +
+      static_cast<int64_t>(h * p.group + col - tok * p.group) * p.o_stride[2] + dim) =
+      make_uint2(pack_bf16x2(v.x * f, v.y * f), pack_bf16x2(v.z * f, v.w * f));
+}
+__device__ __forceinline__ void put_lse(const Kv8AttnParams& p, int b, int h, int col, float m,
+                                        float l) {
+  const int tok = col / p.group;
+  if (tok >= p.rows.tokens) return;
+  p.lse[static_cast<int64_t>(b) * p.lse_stride[0] +
+        static_cast<int64_t>(h * p.group + col - tok * p.group) * p.lse_stride[1] + tok] =
+      l > 0.f ? (m + __log2f(l)) * kLn2 : (l == 0.f ? -INFINITY : l);
+}
+
+// Running (shift of O, max, sum) <- with another part's; returns the factors on both Os.
+__device__ __forceinline__ float2 join(float& m_shift, float& m, float& l, const float4 st) {
+  const float ms = fmaxf(m_shift, st.x), mn = fmaxf(m, st.y);
+  const float fa = m_shift == -INFINITY ? 0.f : ex2(m_shift - ms);
+  const float fb = st.x == -INFINITY ? 0.f : ex2(st.x - ms);
+  l = (m == -INFINITY ? l : l * ex2(m - mn)) + (st.y == -INFINITY ? st.z : st.z * ex2(st.y - mn));
+  m_shift = ms;
+  m = mn;
+  return make_float2(fa, fb);
+}
+
+__device__ __forceinline__ void axpby(float4& v, const float2 f, const float4& o) {
+  v.x = v.x * f.x + o.x * f.y;
+  v.y = v.y * f.x + o.y * f.y;
+  v.z = v.z * f.x + o.z * f.y;
+  v.w = v.w * f.x + o.w * f.y;
+}
 
 }  // namespace
 
-template <int D, bool kInt8>
-__global__ void __launch_bounds__(kKv8Warps * 32, 1) kv8_attn_kernel(const Kv8AttnParams p) {
-  using Cfg = AttnCfg<D>;
+template <typename Cfg, bool kInt8>
+__global__ void __launch_bounds__(Cfg::kThreads, 1) kv8_attn_kernel(const Kv8AttnParams p) {
+  constexpr int D = Cfg::D, kTeam = Cfg::kTeam, kBlocks = Cfg::kBlocks, kCols = Cfg::kCols;
   extern __shared__ __align__(16) uint8_t smem[];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, t = lane & 3;
+  const int team = warp / kTeam, part = warp % kTeam;  // part: which dims
   uint8_t* ring = smem + warp * Cfg::kRing;
-  float4* stats = reinterpret_cast<float4*>(smem + Cfg::kRingBytes);          // [warp][col]
-  int* tails = reinterpret_cast<int*>(smem + Cfg::kRingBytes + kKv8Warps * kKv8Cols * 16);
-  RowPlan* rows = reinterpret_cast<RowPlan*>(smem + Cfg::kRingBytes + Cfg::kStatBytes);
+  float* exchange = reinterpret_cast<float*>(smem + Cfg::kRingBytes);
+  float4* stats = reinterpret_cast<float4*>(smem + Cfg::kRingBytes + Cfg::kExchange);  // [team][col]
+  int* tails = reinterpret_cast<int*>(stats + Cfg::kTeams * kCols);  // [4][team]
+  RowPlan* rows = reinterpret_cast<RowPlan*>(reinterpret_cast<uint8_t*>(tails) +
+                                             ((Cfg::kTails + 15) & ~15));
   int* prefix = reinterpret_cast<int*>(rows + p.rows.batch);
-  int* scan = prefix + p.rows.batch + 1;  // 8 warp sums (+ total)
+  int* scan = prefix + p.rows.batch + 1;
 
   pdl_enter();
   // ---- plan: checked rows, their tiles, the prefix sum over rows ----
   const int B = p.rows.batch, heads = p.cache.heads;
   {
-    const int per = (B + 255) / 256;  // rows per thread, consecutive
+    const int per = (B + Cfg::kThreads - 1) / Cfg::kThreads;  // rows per thread, consecutive
     int mine = 0;
     for (int j = 0; j < per; ++j) {
       const int b = tid * per + j;
       if (b >= B) break;
-      const Kv8Row r = kv8_row(p.cache, p.rows, b, p.max_k);
-      RowPlan rp;
-      rp.slot = r.slot;
-      rp.start = r.start;
-      rp.n = r.n;
-      rp.lo = p.window > 0 ? max(0, r.start - p.window + 1) : 0;
+      const RowPlan rp = row_plan(p, b);
       rows[b] = rp;
-      const int act = active_blocks(rp, p.group);
-      mine += heads * (act * row_tiles(rp) + p.col_blocks - act);
+      const int act = active_groups<kCols>(rp, p.group);
+      mine += heads * (act * row_tiles(rp) + p.col_groups - act);
     }
     int inc = mine;
 #pragma unroll
@@ -161,30 +253,31 @@ __global__ void __launch_bounds__(kKv8Warps * 32, 1) kv8_attn_kernel(const Kv8At
     }
     if (lane == 31) scan[warp] = inc;
     __syncthreads();
-    int before = 0;
-    for (int w = 0; w < warp; ++w) before += scan[w];
-    int at = before + inc - mine;
+    int at = inc - mine;
+    for (int w = 0; w < warp; ++w) at += scan[w];
     for (int j = 0; j < per; ++j) {
       const int b = tid * per + j;
       if (b >= B) break;
       prefix[b] = at;
       const RowPlan rp = rows[b];
-      const int act = active_blocks(rp, p.group);
-      at += heads * (act * row_tiles(rp) + p.col_blocks - act);
+      const int act = active_groups<kCols>(rp, p.group);
+      at += heads * (act * row_tiles(rp) + p.col_groups - act);
       if (b == B - 1) prefix[B] = at;
     }
     __syncthreads();
   }
   const int total = prefix[B];
-  const int n_warps = gridDim.x * kKv8Warps;
-  const int per = (total + n_warps - 1) / n_warps;
-  if (blockIdx.x == 0) {
-    if (tid == 0) p.plan[0] = per;
-    for (int b = tid; b <= B; b += blockDim.x) p.plan[1 + b] = prefix[b];
+  const int runs = min(total, static_cast<int>(gridDim.x) * Cfg::kTeams);
+  if (blockIdx.x == 0) {  // for the merge
+    if (tid == 0) *reinterpret_cast<int4*>(p.plan) = make_int4(runs, total, 0, 0);
+    for (int b = tid; b < B; b += blockDim.x) {
+      reinterpret_cast<int4*>(p.plan)[1 + b] = reinterpret_cast<const int4*>(rows)[b];
+      p.plan[4 + 4 * B + b] = prefix[b];
+    }
   }
-  const int W = blockIdx.x * kKv8Warps + warp;
-  const int w_begin = min(total, W * per), w_end = min(total, w_begin + per);
-  int todo = w_end - w_begin;
+  const int W = blockIdx.x * Cfg::kTeams + team;
+  const int w_begin = W < runs ? run_begin(W, runs, total) : 0;
+  int todo = W < runs ? run_begin(W + 1, runs, total) - w_begin : 0;
 
   // place of a list index
   auto locate = [&](int x) {
@@ -197,7 +290,7 @@ __global__ void __launch_bounds__(kKv8Warps * 32, 1) kv8_attn_kernel(const Kv8At
     pl.b = lo;
     const RowPlan r = rows[lo];
     const int nt = row_tiles(r);
-    const int act = heads * active_blocks(r, p.group);
+    const int act = heads * active_groups<kCols>(r, p.group);
     const int rel = x - prefix[lo];
     if (rel < act * nt) {
       pl.item = rel / nt;
@@ -212,9 +305,8 @@ __global__ void __launch_bounds__(kKv8Warps * 32, 1) kv8_attn_kernel(const Kv8At
     return pl;
   };
   auto next_item = [&](Place& pl) {
-    const RowPlan r = rows[pl.b];
     ++pl.item;
-    if (pl.item >= heads * p.col_blocks) {
+    if (pl.item >= heads * p.col_groups) {
       ++pl.b;
       pl.item = 0;
       if (pl.b >= B) {
@@ -222,92 +314,105 @@ __global__ void __launch_bounds__(kKv8Warps * 32, 1) kv8_attn_kernel(const Kv8At
         return;
       }
     }
-    const RowPlan q = pl.item == 0 ? rows[pl.b] : r;
-    const bool act = pl.item < heads * active_blocks(q, p.group);
-    pl.tile = act ? q.lo / kKv8Tile : 0;
-    pl.left = act ? row_tiles(q) : 1;
+    const RowPlan r = rows[pl.b];
+    const bool act = pl.item < heads * active_groups<kCols>(r, p.group);
+    pl.tile = act ? r.lo / kKv8Tile : 0;
+    pl.left = act ? row_tiles(r) : 1;
   };
-  // KV head and column block of an item
-  auto item_head = [&](const Place& pl, int& head, int& cb) {
-    const int a = active_blocks(rows[pl.b], p.group);
-    if (pl.item < heads * a) {
-      head = pl.item / a;
-      cb = pl.item - head * a;
+  // KV head and column group of an item
+  auto item_head = [&](int b, int item, int& head, int& cg) {
+    const int a = active_groups<kCols>(rows[b], p.group);
+    if (item < heads * a) {
+      head = item / a;
+      cg = item - head * a;
     } else {
-      const int rest = p.col_blocks - a;
-      const int j = pl.item - heads * a;
+      const int rest = p.col_groups - a;
+      const int j = item - heads * a;
       head = j / rest;
-      cb = a + j - head * rest;
+      cg = a + j - head * rest;
     }
   };
 
-  // ---- the loading side: K and V tiles in order K0 V0 K1 V1 ... ----
-  Place ld = locate(todo > 0 ? w_begin : 0);
+  // ---- the loading side: 16-key pieces in order K0a K0b V0a V0b K1a ... ----
+  Place ld = locate(w_begin);
   int ld_todo = todo;        // tiles not yet requested
-  int ld_slot = 0;           // ring buffer of the next request
-  bool ld_v = false;
-  int ld_page = -1, ld_next = -1;
-  int ld_head = 0;
-  int ld_hi = 0;             // one past the last key of the item's row
-  auto lookup = [&](const Place& pl) {
-    const RowPlan r = rows[pl.b];
-    return r.n > 0 && pl.left > 0 ? kv8_page(p.cache, r.slot, pl.tile * kKv8Tile) : -1;
+  uint32_t ld_buf = 0;       // ring offset of the next request
+  int ld_phase = 0;          // 0, 1: K halves; 2, 3: V halves
+  int ld_page[2], ld_next[2];
+  int ld_head = 0, ld_lo = 0, ld_hi = 0, ld_slot = -1;
+  // Page of the 16 keys at `pos`; -1 when no column of the row sees any of them.
+  auto lookup = [&](int pos) {
+    return pos < ld_hi && pos + 16 > ld_lo ? kv8_page(p.cache, ld_slot, pos) : -1;
   };
   auto set_item = [&]() {
-    int cb;
-    item_head(ld, ld_head, cb);
-    ld_hi = rows[ld.b].n > 0 ? rows[ld.b].start + rows[ld.b].n : 0;
+    int cg;
+    item_head(ld.b, ld.item, ld_head, cg);
+    const RowPlan r = rows[ld.b];
+    const bool act = ld.item < heads * active_groups<kCols>(r, p.group);
+    ld_slot = r.slot;
+    ld_lo = r.lo;
+    ld_hi = act ? r.start + r.n : 0;
+    ld_page[0] = lookup(ld.tile * kKv8Tile);
+    ld_page[1] = lookup(ld.tile * kKv8Tile + 16);
   };
-  if (todo > 0) {
-    set_item();
-    ld_page = lookup(ld);
-  }
+  if (todo > 0) set_item();
+  // lane's place in a piece: kDims / 16 lanes per row
+  constexpr int kLanesRow = Cfg::kDims / 16, kRowsStep = 32 / kLanesRow;
+  const uint32_t ring_s = smem_addr(ring);
+  const uint32_t ld_dst = (lane / kLanesRow) * Cfg::kRow + (lane % kLanesRow) * 16;
+  const int ld_src = (lane / kLanesRow) * D + part * Cfg::kDims + (lane % kLanesRow) * 16;
   auto request = [&]() {
     if (ld_todo > 0) {
-      const int pos = ld.tile * kKv8Tile;
-      uint8_t* buf = ring + ld_slot * Cfg::kBuf;
-      const uint32_t dst = smem_addr(buf);
-      const int page = ld_page;
+      const int half = ld_phase & 1;
+      const bool is_v = ld_phase >= 2;
+      const int pos = ld.tile * kKv8Tile + half * 16;
+      const int page = ld_page[half];
       const int64_t block = static_cast<int64_t>(max(page, 0)) * heads + ld_head;
-      const uint8_t* src = (ld_v ? p.cache.v : p.cache.k) +
+      const uint8_t* src = (is_v ? p.cache.v : p.cache.k) + ld_src +
                            (block * p.cache.page + (pos & (p.cache.page - 1))) * D;
-      const int rows_ok = page >= 0 ? min(kKv8Tile, ld_hi - pos) : 0;
-      if constexpr (D == 512) {
+      const uint32_t dst = ring_s + ld_buf + ld_dst;
+      const int rows_ok = page >= 0 ? ld_hi - pos : 0;
+      if (rows_ok >= 16) {
 #pragma unroll
-        for (int j = 0; j < 16; ++j)
-          cp16(dst + j * Cfg::kRow + lane * 16, src + j * 512 + lane * 16, j < rows_ok ? 16 : 0);
-      } else {
+        for (int j = 0; j < 16 / kRowsStep; ++j)
+          cp16(dst + j * kRowsStep * Cfg::kRow, src + j * kRowsStep * D);
+      } else {  // zeros in rows past the end, or everywhere
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const int row = 2 * j + (lane >> 4);
-          cp16(dst + row * Cfg::kRow + (lane & 15) * 16, src + j * 512 + lane * 16,
-               row < rows_ok ? 16 : 0);
+        for (int j = 0; j < 16 / kRowsStep; ++j)
+          cp16_z(dst + j * kRowsStep * Cfg::kRow, src + j * kRowsStep * D,
+                 j * kRowsStep + lane / kLanesRow < rows_ok ? 16 : 0);
+      }
+      if (lane == 0 && ld_phase != 3) {
+        // a piece's scale and page id ride in its first row's padding; V's second
+        // scale comes with the first half, since P needs both
+        cp4_z(ring_s + ld_buf + Cfg::kDims,
+              (is_v ? p.cache.v_scale : p.cache.k_scale) + block, page >= 0 ? 4 : 0);
+        *reinterpret_cast<int*>(ring + ld_buf + Cfg::kDims + 4) = page;
+        if (is_v) {
+          const int page1 = ld_page[1];
+          cp4_z(ring_s + ld_buf + Cfg::kDims + 8,
+                p.cache.v_scale + static_cast<int64_t>(max(page1, 0)) * heads + ld_head,
+                page1 >= 0 ? 4 : 0);
         }
       }
-      if (lane == 0) {  // the block's scale and the page id ride in the first row's padding
-        cp4(dst + D, (ld_v ? p.cache.v_scale : p.cache.k_scale) + block, page >= 0 ? 4 : 0);
-        *reinterpret_cast<int*>(buf + D + 4) = page;
+      if (ld_phase == 0) {  // look the next tile's pages up one tile ahead
+        const int np = pos + kKv8Tile;
+        ld_next[0] = ld.left > 1 ? lookup(np) : -1;
+        ld_next[1] = ld.left > 1 ? lookup(np + 16) : -1;
       }
-      if (ld_v) {
+      if (ld_phase == 3) {
         --ld_todo;
         ++ld.tile;
         if (--ld.left == 0) {
           next_item(ld);
-          if (ld_todo > 0) {
-            set_item();
-            ld_page = lookup(ld);
-          }
+          if (ld_todo > 0) set_item();
         } else {
-          ld_page = ld_next;
+          ld_page[0] = ld_next[0];
+          ld_page[1] = ld_next[1];
         }
-      } else {  // look the next tile's page up one tile ahead
-        Place nx = ld;
-        ++nx.tile;
-        --nx.left;
-        ld_next = ld_todo > 1 ? lookup(nx) : -1;
       }
-      ld_v = !ld_v;
-      ld_slot = ld_slot + 1 == Cfg::kBufs ? 0 : ld_slot + 1;
+      ld_phase = (ld_phase + 1) & 3;
+      ld_buf = ld_buf + Cfg::kBuf == Cfg::kRing ? 0 : ld_buf + Cfg::kBuf;
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
@@ -315,154 +420,147 @@ __global__ void __launch_bounds__(kKv8Warps * 32, 1) kv8_attn_kernel(const Kv8At
   for (int i = 0; i < Cfg::kBufs; ++i) request();
 
   // ---- the computing side ----
-  uint32_t qf[Cfg::kChunks][8];
-  float acc[Cfg::kAcc / 4][4];
-  float m_o[2], m_s[2], l_s[2];  // per column 2t, 2t + 1: shift of O; max and partial sum of P
-  float q_back[2];               // log2(e) * 2^-e of the column's Q
-  Place pl = locate(todo > 0 ? w_begin : 0);
-  int use_slot = 0;
-  int head = 0, cb = 0;
+  uint32_t qf[kBlocks][Cfg::kChunks][8];
+  float acc[kBlocks][Cfg::kTilesM][4];
+  float m_o[kBlocks][2], m_s[kBlocks][2], l_s[kBlocks][2];  // per column 2t, 2t + 1 of a block:
+                                                            // shift of O; max and sum of P
+  float q_back[kBlocks][2];               // log2(e) * 2^-e of the column's Q
+  int last_key[kBlocks][2];               // last visible key, -1: a padded column
+  Place pl = locate(w_begin);
+  uint32_t use = 0;                       // ring offset of the next piece
+  int head = 0, cg = 0, swap = 0;
 
   auto begin_item = [&]() {
-    item_head(pl, head, cb);
+    item_head(pl.b, pl.item, head, cg);
     const RowPlan r = rows[pl.b];
-    // this thread's Q fragments: column g, dims of chunk c(t, i)
-    const int col = cb * kKv8Cols + g;
-    const int tok = col / p.group;
-    const bool have = tok < r.n;
-    const __nv_bfloat16* qp =
-        p.q + static_cast<int64_t>(pl.b) * p.q_stride[0] +
-        static_cast<int64_t>(have ? tok : 0) * p.q_stride[1] +
-        static_cast<int64_t>(head * p.group + (have ? col - tok * p.group : 0)) * p.q_stride[2];
-    uint4 raw[Cfg::kChunks][2];
-    float amax = 0.f;
 #pragma unroll
-    for (int i = 0; i < Cfg::kChunks; ++i) {
-      const int c = 2 * t + (i & 1) + 8 * (i >> 1);
-      const uint4* s = reinterpret_cast<const uint4*>(qp + c * 16);
-      raw[i][0] = have ? s[0] : make_uint4(0u, 0u, 0u, 0u);
-      raw[i][1] = have ? s[1] : make_uint4(0u, 0u, 0u, 0u);
-    }
+    for (int bl = 0; bl < kBlocks; ++bl) {
+      // this thread's Q fragments: column g, dims of chunk c(t, i)
+      const int col = cg * kCols + bl * 8 + g;
+      const int tok = col / p.group;
+      const bool have = tok < r.n;
+      const __nv_bfloat16* qp =
+          p.q + static_cast<int64_t>(pl.b) * p.q_stride[0] +
+          static_cast<int64_t>(have ? tok : 0) * p.q_stride[1] +
+          static_cast<int64_t>(head * p.group + (have ? col - tok * p.group : 0)) * p.q_stride[2];
+      // its raw values, and the column's largest magnitude over all D dims (the other
+      // warps' dims too, so that every warp of the team finds the same one)
+      uint4 raw[Cfg::kChunks][2];
+      uint32_t top = 0;
 #pragma unroll
-    for (int i = 0; i < Cfg::kChunks; ++i) {
+      for (int w = 0; w < kTeam; ++w) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const uint32_t w[4] = {raw[i][h].x, raw[i][h].y, raw[i][h].z, raw[i][h].w};
+        for (int i = 0; i < Cfg::kChunks; ++i) {
+          const uint4* s = reinterpret_cast<const uint4*>(
+              qp + (part ^ (kTeam - 1 - w)) * Cfg::kDims + (2 * t + (i & 1) + 8 * (i >> 1)) * 16);
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          amax = fmaxf(amax, fabsf(__uint_as_float(w[x] << 16)));
-          amax = fmaxf(amax, fabsf(__uint_as_float(w[x] & 0xffff0000u)));
+          for (int h = 0; h < 2; ++h) {
+            raw[i][h] = have ? s[h] : make_uint4(0u, 0u, 0u, 0u);
+            const uint4 x = raw[i][h];
+            top = __vmaxu2(__vmaxu2(top, x.x & 0x7fff7fffu), x.y & 0x7fff7fffu);
+            top = __vmaxu2(__vmaxu2(top, x.z & 0x7fff7fffu), x.w & 0x7fff7fffu);
+          }
         }
       }
-    }
-    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-    const int e = q_exponent(amax);
-    // two factors: 2^e alone may leave the fp32 range for the smallest inputs
-    const float f1 = __uint_as_float(static_cast<uint32_t>(127 + e / 2) << 23);
-    const float f2 = __uint_as_float(static_cast<uint32_t>(127 + e - e / 2) << 23);
+      top = max(top >> 16, top & 0xffffu);
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      const int e = q_exponent(__uint_as_float(top << 16));
+      // two factors: 2^e alone may leave the fp32 range for the smallest inputs
+      const float f1 = __uint_as_float(static_cast<uint32_t>(127 + e / 2) << 23);
+      const float f2 = __uint_as_float(static_cast<uint32_t>(127 + e - e / 2) << 23);
 #pragma unroll
-    for (int i = 0; i < Cfg::kChunks; ++i) {
+      for (int i = 0; i < Cfg::kChunks; ++i) {
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const uint32_t w[4] = {raw[i][h].x, raw[i][h].y, raw[i][h].z, raw[i][h].w};
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t w[4] = {raw[i][h].x, raw[i][h].y, raw[i][h].z, raw[i][h].w};
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-          const float lo = __uint_as_float(w[x] << 16) * f1 * f2;
-          const float hi = __uint_as_float(w[x] & 0xffff0000u) * f1 * f2;
-          const __half2 v = __floats2half2_rn(lo, hi);
-          qf[i][4 * h + x] = *reinterpret_cast<const uint32_t*>(&v);
+          for (int x = 0; x < 4; ++x) {
+            const float lo = __uint_as_float(w[x] << 16) * f1 * f2;
+            const float hi = __uint_as_float(w[x] & 0xffff0000u) * f1 * f2;
+            const __half2 v = __floats2half2_rn(lo, hi);
+            qf[bl][i][4 * h + x] = *reinterpret_cast<const uint32_t*>(&v);
+          }
         }
       }
-    }
 #pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      const int ce = __shfl_sync(0xffffffffu, e, (2 * t + x) * 4);  // column 2t + x
-      q_back[x] = kLog2e * __uint_as_float(static_cast<uint32_t>(127 - ce) << 23);
-      m_o[x] = m_s[x] = -INFINITY;
-      l_s[x] = 0.f;
-    }
+      for (int x = 0; x < 2; ++x) {
+        const int ce = __shfl_sync(0xffffffffu, e, (2 * t + x) * 4);  // column 2t + x
+        q_back[bl][x] = kLog2e * __uint_as_float(static_cast<uint32_t>(127 - ce) << 23);
+        const int ct = (cg * kCols + bl * 8 + 2 * t + x) / p.group;
+        last_key[bl][x] = ct < r.n ? r.start + ct : -1;
+        m_o[bl][x] = m_s[bl][x] = -INFINITY;
+        l_s[bl][x] = 0.f;
+      }
 #pragma unroll
-    for (int i = 0; i < Cfg::kAcc / 4; ++i)
+      for (int i = 0; i < Cfg::kTilesM; ++i)
 #pragma unroll
-      for (int x = 0; x < 4; ++x) acc[i][x] = 0.f;
-  };
-
-  // Sum over the warp's rows of a column's partial sums.
-  auto column_sums = [&]() {
-#pragma unroll
-    for (int x = 0; x < 2; ++x) {
-#pragma unroll
-      for (int o = 4; o < 32; o <<= 1) l_s[x] += __shfl_xor_sync(0xffffffffu, l_s[x], o);
+        for (int x = 0; x < 4; ++x) acc[bl][i][x] = 0.f;
     }
   };
-  auto slot_store = [&](int which) {  // raw partial of this warp (0 head, 1 tail)
-    const int64_t s = 2 * static_cast<int64_t>(W) + which;
-    float* po = p.part_o + s * (D * kKv8Cols);
-    const int cols = p.rows.tokens * p.group - cb * kKv8Cols;
-    if (2 * t < cols) {
+  auto column_sums = [&]() {  // over the warp's key rows
 #pragma unroll
-      for (int i = 0; i < Cfg::kAcc / 4; ++i)
-#pragma unroll
-        for (int x = 0; x < 4; ++x) po[(i * 4 + x) * 32 + lane] = acc[i][x];
-    }
-    if (g == 0) {
+    for (int bl = 0; bl < kBlocks; ++bl)
 #pragma unroll
       for (int x = 0; x < 2; ++x)
-        p.part_ml[s * kKv8Cols + 2 * t + x] = make_float4(m_o[x], m_s[x], l_s[x], 0.f);
-    }
-  };
-  // 16 consecutive dims of one column
-  auto put = [&](int b, int h, int block, int col8, int step, int gg, const float (&v)[16],
-                 float f) {
-    const int col = block * kKv8Cols + col8;
-    const int tok = col / p.group;
-    if (tok >= p.rows.tokens) return;
-    uint32_t w[8];
 #pragma unroll
-    for (int x = 0; x < 8; ++x) w[x] = pack_bf16x2(v[2 * x] * f, v[2 * x + 1] * f);
-    uint4* dst = reinterpret_cast<uint4*>(
-        p.o + static_cast<int64_t>(b) * p.o_stride[0] + static_cast<int64_t>(tok) * p.o_stride[1] +
-        static_cast<int64_t>(h * p.group + col - tok * p.group) * p.o_stride[2] +
-        v_chunk(gg, step) * 16);
-    dst[0] = make_uint4(w[0], w[1], w[2], w[3]);
-    dst[1] = make_uint4(w[4], w[5], w[6], w[7]);
+        for (int o = 4; o < 32; o <<= 1)
+          l_s[bl][x] += __shfl_xor_sync(0xffffffffu, l_s[bl][x], o);
   };
-  auto put_lse = [&](int b, int h, int block, int col8, float m, float l) {
-    const int col = block * kKv8Cols + col8;
-    const int tok = col / p.group;
-    if (tok >= p.rows.tokens) return;
-    p.lse[static_cast<int64_t>(b) * p.lse_stride[0] +
-          static_cast<int64_t>(h * p.group + col - tok * p.group) * p.lse_stride[1] + tok] =
-        l > 0.f ? (m + __log2f(l)) * kLn2 : (l == 0.f ? -INFINITY : l);
-  };
-  auto out_factor = [&](float m_shift, float m, float l) {
-    // O is held as sum * 2^(kShiftUp - m_shift); without a visible key it is zero
-    return l == 0.f || m_shift == -INFINITY ? 0.f : ex2(m_shift - kShiftUp - m) / l;
-  };
-  auto finish = [&]() {  // the whole item lies in this warp's run
+  // A partial O is [column][dim]; padded columns are left out.  (In shared memory the
+  // column stride and the order of the four stores keep a quarter-warp's banks apart.)
+  auto store_part = [&](float* po, int stride, float4* ml, int cols) {
 #pragma unroll
-    for (int x = 0; x < 2; ++x) {
-      const float f = out_factor(m_o[x], m_s[x], l_s[x]);
+    for (int bl = 0; bl < kBlocks; ++bl)
 #pragma unroll
-      for (int i = 0; i < Cfg::kSteps; ++i) {
-        float v[16];
+      for (int x = 0; x < 2; ++x) {
+        const int col = bl * 8 + 2 * t + x;
+        if (col < cols) {
 #pragma unroll
-        for (int y = 0; y < 8; ++y) {
-          v[2 * y] = acc[i * 8 + y][x];
-          v[2 * y + 1] = acc[i * 8 + y][2 + x];
+          for (int i = 0; i < Cfg::kSteps; ++i) {
+            float4* dst = reinterpret_cast<float4*>(po + col * stride + part * Cfg::kDims +
+                                                    v_chunk(g, i) * 16);
+            const auto quad = [&](int y) {
+              return make_float4(acc[bl][i * 8 + 2 * y][x], acc[bl][i * 8 + 2 * y][2 + x],
+                                 acc[bl][i * 8 + 2 * y + 1][x],
+                                 acc[bl][i * 8 + 2 * y + 1][2 + x]);
+            };
+#pragma unroll
+            for (int y = 0; y < 4; ++y) dst[y ^ (g & 1)] = (g & 1) ? quad(y ^ 1) : quad(y);
+          }
+          if (g == 0 && part == 0)
+            ml[col] = make_float4(m_o[bl][x], m_s[bl][x], l_s[bl][x], 0.f);
         }
-        put(pl.b, head, cb, 2 * t + x, i, g, v, f);
       }
-      if (g == 0) put_lse(pl.b, head, cb, 2 * t + x, m_s[x], l_s[x]);
+  };
+  auto finish = [&]() {  // the whole item lies in this run
+#pragma unroll
+    for (int bl = 0; bl < kBlocks; ++bl) {
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const int col = cg * kCols + bl * 8 + 2 * t + x;
+        const float f = out_factor(m_o[bl][x], m_s[bl][x], l_s[bl][x]);
+#pragma unroll
+        for (int i = 0; i < Cfg::kSteps; ++i) {
+          float v[16];
+#pragma unroll
+          for (int y = 0; y < 8; ++y) {
+            v[2 * y] = acc[bl][i * 8 + y][x];
+            v[2 * y + 1] = acc[bl][i * 8 + y][2 + x];
+          }
+          put_out(p, pl.b, head, col, part * Cfg::kDims + v_chunk(g, i) * 16, v, f);
+        }
+        if (g == 0 && part == 0) put_lse(p, pl.b, head, col, m_s[bl][x], l_s[bl][x]);
+      }
     }
   };
 
   bool open = false;           // an item is in progress
   bool from_start = false;     // its first tile lies in this run
   if (todo > 0) {
-    from_start = pl.left == (pl.item < heads * active_blocks(rows[pl.b], p.group)
-                                 ? row_tiles(rows[pl.b]) : 1);
+    const RowPlan r = rows[pl.b];
+    from_start =
+        pl.left == (pl.item < heads * active_groups<kCols>(r, p.group) ? row_tiles(r) : 1);
   }
 #pragma unroll 1
   while (todo > 0) {
@@ -470,17 +568,26 @@ __global__ void __launch_bounds__(kKv8Warps * 32, 1) kv8_attn_kernel(const Kv8At
       begin_item();
       open = true;
     }
-    const RowPlan r = rows[pl.b];
-    // ---- S^T of the tile ----
-    asm volatile("cp.async.wait_group %0;" ::"n"(Cfg::kBufs - 1) : "memory");
-    __syncwarp();
-    float s[2][4];
+    // ---- S^T of the tile, through shared memory: rows g and g + 8 of both halves ----
+    float k_scale[2];
+    bool page_ok[2];
+    float* mine = exchange + (swap * Cfg::kWarps + warp) * (kBlocks * 256) + lane;
+#pragma unroll 1
+    for (int half = 0; half < 2; ++half) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(Cfg::kBufs - 1) : "memory");
+      __syncwarp();
+      const uint8_t* kb = ring + use;
+      const float sc = *reinterpret_cast<const float*>(kb + Cfg::kDims);
+      const bool ok = *reinterpret_cast<const int*>(kb + Cfg::kDims + 4) >= 0;
+      k_scale[0] = half == 0 ? sc : k_scale[0];
+      page_ok[0] = half == 0 ? ok : page_ok[0];
+      k_scale[1] = sc;
+      page_ok[1] = ok;
+      float c[2][kBlocks][4];
 #pragma unroll
-    for (int x = 0; x < 4; ++x) s[0][x] = s[1][x] = 0.f;
-    const uint8_t* kb = ring + use_slot * Cfg::kBuf;
-    const float k_scale = *reinterpret_cast<const float*>(kb + D);
-    const int page = *reinterpret_cast<const int*>(kb + D + 4);
-    {
+      for (int bl = 0; bl < kBlocks; ++bl)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) c[0][bl][x] = c[1][bl][x] = 0.f;
       const uint8_t* r0 = kb + g * Cfg::kRow + 32 * t;
 #pragma unroll
       for (int i = 0; i < Cfg::kChunks; ++i) {
@@ -493,88 +600,139 @@ __global__ void __launch_bounds__(kKv8Warps * 32, 1) kv8_attn_kernel(const Kv8At
           uint32_t a[4];
           kv8_to_half<kInt8>(xw[j], a[0], a[2]);
           kv8_to_half<kInt8>(yw[j], a[1], a[3]);
-          mma_16816(s[j & 1], a, qf[i][2 * j], qf[i][2 * j + 1]);
+#pragma unroll
+          for (int bl = 0; bl < kBlocks; ++bl)
+            mma_16816(c[kBlocks == 1 ? j & 1 : 0][bl], a, qf[bl][i][2 * j], qf[bl][i][2 * j + 1]);
         }
       }
+#pragma unroll
+      for (int bl = 0; bl < kBlocks; ++bl)
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+          mine[((half * kBlocks + bl) * 4 + x) * 32] =
+              kBlocks == 1 ? c[0][bl][x] + c[1][bl][x] : c[0][bl][x];
+      __syncwarp();
+      request();
+      use = use + Cfg::kBuf == Cfg::kRing ? 0 : use + Cfg::kBuf;
     }
-    __syncwarp();
-    request();
-    use_slot = use_slot + 1 == Cfg::kBufs ? 0 : use_slot + 1;
+    if constexpr (kTeam > 1)
+      asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "n"(32 * kTeam) : "memory");
+    float s[2][kBlocks][4];
+    {  // the team's partial sums, added in the same order by all
+      const float* all = exchange + (swap * Cfg::kWarps + team * kTeam) * (kBlocks * 256) + lane;
+#pragma unroll
+      for (int half = 0; half < 2; ++half)
+#pragma unroll
+        for (int bl = 0; bl < kBlocks; ++bl)
+#pragma unroll
+          for (int x = 0; x < 4; ++x) {
+            const int at = ((half * kBlocks + bl) * 4 + x) * 32;
+            float sum = all[at];
+#pragma unroll
+            for (int w = 1; w < kTeam; ++w) sum += all[w * (kBlocks * 256) + at];
+            s[half][bl][x] = sum;
+          }
+      if constexpr (kTeam > 1) swap ^= 1;
+    }
 
     // ---- mask, running maxima, P ----
     asm volatile("cp.async.wait_group %0;" ::"n"(Cfg::kBufs - 1) : "memory");
     __syncwarp();
-    const uint8_t* vb = ring + use_slot * Cfg::kBuf;
-    const float v_scale = *reinterpret_cast<const float*>(vb + D);
-    const int v_exp = static_cast<int>((__float_as_uint(v_scale) >> 23) & 255u) - 127;
-    const float v_mant = v_exp == -127 ? 0.f
-                                       : __uint_as_float((__float_as_uint(v_scale) & 0x807fffffu) |
-                                                         0x3f800000u);
-    uint32_t pk[2];  // P of keys g and g + 8, columns 2t and 2t + 1
+    float v_exp[2], v_mant[2];
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const uint32_t bits =
+          *reinterpret_cast<const uint32_t*>(ring + use + Cfg::kDims + 8 * half);
+      const int e = static_cast<int>((bits >> 23) & 255u) - 127;
+      v_exp[half] = static_cast<float>(e);
+      v_mant[half] = e == -127 ? 0.f : __uint_as_float((bits & 0x807fffffu) | 0x3f800000u);
+    }
+    uint32_t pf[2][kBlocks][2];  // P^T as B operands: column g, keys t, t + 4, t + 8, t + 12
     bool rescale = false;
-    float alpha[2];
-    {
-      float pv[2][2];
+    float alpha[kBlocks][2];
+    const int k_first = pl.tile * kKv8Tile + g;
+#pragma unroll
+    for (int bl = 0; bl < kBlocks; ++bl) {
+      uint32_t pk[2][2];         // [half][rows g, g + 8], columns 2t and 2t + 1
+      float pv[2][2][2];         // [column][half][row]
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
-        const int tok = (cb * kKv8Cols + 2 * t + x) / p.group;
-        const int q_pos = r.start + tok;
-        float z[2];
+        const int hi = last_key[bl][x];
+        const int lo = p.window > 0 ? hi - p.window : -1;    // keys > lo are visible
+        float z[2][2];
 #pragma unroll
-        for (int y = 0; y < 2; ++y) {
-          const int k_pos = pl.tile * kKv8Tile + g + 8 * y;
-          const bool seen = page >= 0 && tok < r.n && k_pos <= q_pos &&
-                            (p.window == 0 || k_pos > q_pos - p.window);
-          z[y] = seen ? (s[0][2 * y + x] + s[1][2 * y + x]) * (k_scale * q_back[x]) : -INFINITY;
+        for (int half = 0; half < 2; ++half)
+#pragma unroll
+          for (int y = 0; y < 2; ++y) {
+            const int k = k_first + half * 16 + y * 8;
+            z[half][y] = page_ok[half] && k <= hi && k > lo
+                             ? s[half][bl][2 * y + x] * (k_scale[half] * q_back[bl][x])
+                             : -INFINITY;
+          }
+        float top = fmaxf(z[0][0], z[0][1]), top1 = fmaxf(z[1][0], z[1][1]);
+        float top_v = fmaxf(top + v_exp[0], top1 + v_exp[1]);
+        top = fmaxf(top, top1);
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) {
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+          top_v = fmaxf(top_v, __shfl_xor_sync(0xffffffffu, top_v, o));
         }
-        float top = fmaxf(z[0], z[1]);
-#pragma unroll
-        for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        const float m_new = fmaxf(m_s[x], top);
+        const float m_new = fmaxf(m_s[bl][x], top);
         const float m_use = m_new == -INFINITY ? 0.f : m_new;
-        l_s[x] = l_s[x] * ex2(m_s[x] - m_use) + ex2(z[0] - m_use) + ex2(z[1] - m_use);
-        m_s[x] = m_new;
-        alpha[x] = 1.f;
-        const float top_v = top + static_cast<float>(v_exp);
-        if (top_v > m_o[x] + kStale) {  // also the first visible key
-          alpha[x] = m_o[x] == -INFINITY ? 0.f : ex2(m_o[x] - top_v);
-          m_o[x] = top_v;
+        l_s[bl][x] = l_s[bl][x] * ex2(m_s[bl][x] - m_use) +
+                     ((ex2(z[0][0] - m_use) + ex2(z[0][1] - m_use)) +
+                      (ex2(z[1][0] - m_use) + ex2(z[1][1] - m_use)));
+        m_s[bl][x] = m_new;
+        alpha[bl][x] = 1.f;
+        if (top_v > m_o[bl][x] + kStale) {  // also the first visible key
+          alpha[bl][x] = m_o[bl][x] == -INFINITY ? 0.f : ex2(m_o[bl][x] - top_v);
+          m_o[bl][x] = top_v;
           rescale = true;
         }
-        const float m_sub = (m_o[x] == -INFINITY ? 0.f : m_o[x]) - static_cast<float>(v_exp) -
-                            kShiftUp;
-        pv[x][0] = ex2(z[0] - m_sub) * v_mant;
-        pv[x][1] = ex2(z[1] - m_sub) * v_mant;
+        const float m_sub = (m_o[bl][x] == -INFINITY ? 0.f : m_o[bl][x]) - kShiftUp;
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+#pragma unroll
+          for (int y = 0; y < 2; ++y)
+            pv[x][half][y] = ex2(z[half][y] + v_exp[half] - m_sub) * v_mant[half];
       }
 #pragma unroll
-      for (int y = 0; y < 2; ++y) {
-        const __half2 v = __floats2half2_rn(pv[0][y], pv[1][y]);
-        pk[y] = *reinterpret_cast<const uint32_t*>(&v);
+      for (int half = 0; half < 2; ++half) {
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          const __half2 v = __floats2half2_rn(pv[0][half][y], pv[1][half][y]);
+          pk[half][y] = *reinterpret_cast<const uint32_t*>(&v);
+        }
+        const uint32_t sel = (g & 1) ? 0x7632u : 0x5410u;
+#pragma unroll
+        for (int y = 0; y < 2; ++y) {
+          const uint32_t x0 = __shfl_sync(0xffffffffu, pk[half][y], t * 4 + (g >> 1));
+          const uint32_t x1 = __shfl_sync(0xffffffffu, pk[half][y], (t + 4) * 4 + (g >> 1));
+          pf[half][bl][y] = __byte_perm(x0, x1, sel);
+        }
       }
     }
     if (__any_sync(0xffffffffu, rescale)) {
 #pragma unroll
-      for (int i = 0; i < Cfg::kAcc / 4; ++i) {
-        acc[i][0] *= alpha[0];
-        acc[i][1] *= alpha[1];
-        acc[i][2] *= alpha[0];
-        acc[i][3] *= alpha[1];
-      }
-    }
-    // P^T as the B operand: column g, keys t, t + 4, t + 8, t + 12
-    uint32_t b0, b1;
-    {
-      const uint32_t x0 = __shfl_sync(0xffffffffu, pk[0], t * 4 + (g >> 1));
-      const uint32_t x1 = __shfl_sync(0xffffffffu, pk[0], (t + 4) * 4 + (g >> 1));
-      const uint32_t x2 = __shfl_sync(0xffffffffu, pk[1], t * 4 + (g >> 1));
-      const uint32_t x3 = __shfl_sync(0xffffffffu, pk[1], (t + 4) * 4 + (g >> 1));
-      const uint32_t sel = (g & 1) ? 0x7632u : 0x5410u;
-      b0 = __byte_perm(x0, x1, sel);
-      b1 = __byte_perm(x2, x3, sel);
+      for (int bl = 0; bl < kBlocks; ++bl)
+#pragma unroll
+        for (int i = 0; i < Cfg::kTilesM; ++i) {
+          acc[bl][i][0] *= alpha[bl][0];
+          acc[bl][i][1] *= alpha[bl][1];
+          acc[bl][i][2] *= alpha[bl][0];
+          acc[bl][i][3] *= alpha[bl][1];
+        }
     }
     // ---- O^T += V^T P^T ----
-    {
-      const uint8_t* r0 = vb + t * Cfg::kRow;
+#pragma unroll 1
+    for (int half = 0; half < 2; ++half) {
+      uint32_t pb[kBlocks][2];
+#pragma unroll
+      for (int bl = 0; bl < kBlocks; ++bl) {
+        pb[bl][0] = half == 0 ? pf[0][bl][0] : pf[1][bl][0];
+        pb[bl][1] = half == 0 ? pf[0][bl][1] : pf[1][bl][1];
+      }
+      const uint8_t* r0 = ring + use + t * Cfg::kRow;
 #pragma unroll
       for (int i = 0; i < Cfg::kSteps; ++i) {
         const int off = v_chunk(g, i) * 16;
@@ -593,14 +751,20 @@ __global__ void __launch_bounds__(kKv8Warps * 32, 1) kv8_attn_kernel(const Kv8At
           kv8_to_half<kInt8>(__byte_perm(w[2][y], w[3][y], 0x5140), a[2], a[3]);
           kv8_to_half<kInt8>(__byte_perm(w[0][y], w[1][y], 0x7362), c[0], c[1]);
           kv8_to_half<kInt8>(__byte_perm(w[2][y], w[3][y], 0x7362), c[2], c[3]);
-          mma_16816(acc[i * 8 + 2 * y], a, b0, b1);
-          mma_16816(acc[i * 8 + 2 * y + 1], c, b0, b1);
+#pragma unroll
+          for (int bl = 0; bl < kBlocks; ++bl) {
+            mma_16816(acc[bl][i * 8 + 2 * y], a, pb[bl][0], pb[bl][1]);
+            mma_16816(acc[bl][i * 8 + 2 * y + 1], c, pb[bl][0], pb[bl][1]);
+          }
         }
       }
+      __syncwarp();
+      request();
+      use = use + Cfg::kBuf == Cfg::kRing ? 0 : use + Cfg::kBuf;
+      // the second half's codes (after it, the next tile's, which it waits for anyway)
+      asm volatile("cp.async.wait_group %0;" ::"n"(Cfg::kBufs - 1) : "memory");
+      __syncwarp();
     }
-    __syncwarp();
-    request();
-    use_slot = use_slot + 1 == Cfg::kBufs ? 0 : use_slot + 1;
 
     --todo;
     ++pl.tile;
@@ -609,9 +773,11 @@ __global__ void __launch_bounds__(kKv8Warps * 32, 1) kv8_attn_kernel(const Kv8At
         column_sums();
         finish();
         open = false;
-      } else if (todo > 0) {  // began in an earlier run, ends inside this one
+      } else if (todo > 0) {
         column_sums();
-        slot_store(0);
+        const int64_t sl = 2 * static_cast<int64_t>(W);
+        store_part(p.part_o + sl * Cfg::kOut, D, p.part_ml + sl * kCols,
+                   p.rows.tokens * p.group - cg * kCols);
         open = false;
       }
       if (!open) {
@@ -621,211 +787,198 @@ __global__ void __launch_bounds__(kKv8Warps * 32, 1) kv8_attn_kernel(const Kv8At
     }
   }
 
-  // ---- the runs' ends: sum what belongs to one item over the CTA's warps ----
-  // tails, one per warp each: item key (-1 none), starts in the run, ends in it, row
+  // ---- the runs' ends: sum what belongs to one item over the CTA's teams ----
   asm volatile("cp.async.wait_group 0;" ::: "memory");
   __syncthreads();  // every warp's ring is free
   if (open) column_sums();
-  if (lane == 0) {
-    tails[warp] = open ? pl.b * (heads * p.col_blocks) + pl.item : -1;
-    tails[8 + warp] = from_start;
-    tails[16 + warp] = pl.left == 0;
-    tails[24 + warp] = pl.b;
+  // tails, one per team each: item key (-1 none), starts in the run, ends in it, row
+  if (lane == 0 && part == 0) {
+    tails[team] = open ? pl.b * (heads * p.col_groups) + pl.item : -1;
+    tails[Cfg::kTeams + team] = from_start;
+    tails[2 * Cfg::kTeams + team] = pl.left == 0;
+    tails[3 * Cfg::kTeams + team] = pl.b;
   }
-  float* osh = reinterpret_cast<float*>(smem);  // [warp][register][lane]
+  __syncthreads();
+  float* osh = reinterpret_cast<float*>(smem);  // [team][column] partial O
   if (open) {
-#pragma unroll
-    for (int i = 0; i < Cfg::kAcc / 4; ++i)
-#pragma unroll
-      for (int x = 0; x < 4; ++x)
-        osh[warp * (D * kKv8Cols) + (i * 4 + x) * 32 + lane] = acc[i][x];
-    if (g == 0) {
-#pragma unroll
-      for (int x = 0; x < 2; ++x)
-        stats[warp * kKv8Cols + 2 * t + x] = make_float4(m_o[x], m_s[x], l_s[x], 0.f);
+    const int key = tails[team];
+    const bool alone = (team == 0 || tails[team - 1] != key) &&
+                       (team == Cfg::kTeams - 1 || tails[team + 1] != key);
+    if (alone) {  // nothing to add in this CTA
+      const int64_t sl = 2 * static_cast<int64_t>(W) + 1;
+      store_part(p.part_o + sl * Cfg::kOut, D, p.part_ml + sl * kCols,
+                 p.rows.tokens * p.group - cg * kCols);
+    } else {
+      store_part(osh + team * kCols * Cfg::kOutRow, Cfg::kOutRow, stats + team * kCols, kCols);
     }
   }
   __syncthreads();
-  for (int w0 = 0; w0 < kKv8Warps;) {
+  for (int w0 = 0; w0 < Cfg::kTeams;) {
     const int key = tails[w0];
     if (key < 0) {
       ++w0;
       continue;
     }
     int w1 = w0 + 1;
-    while (w1 < kKv8Warps && tails[w1] == key) ++w1;
-    const bool whole = tails[8 + w0] && tails[16 + w1 - 1];
-    Place it;
-    it.b = tails[24 + w0];
-    it.item = key - it.b * (heads * p.col_blocks);
-    int h, block;
-    item_head(it, h, block);
-    // thread: step, column of a lane's pair, lane
-    for (int u = tid; u < Cfg::kSteps * 64; u += blockDim.x) {
-      const int ln = u & 31, x = (u >> 5) & 1, i = u >> 6;
-      const int col8 = 2 * (ln & 3) + x;
+    while (w1 < Cfg::kTeams && tails[w1] == key) ++w1;
+    if (w1 == w0 + 1) {
+      w0 = w1;
+      continue;
+    }
+    const bool whole = tails[Cfg::kTeams + w0] && tails[2 * Cfg::kTeams + w1 - 1];
+    const int b = tails[3 * Cfg::kTeams + w0];
+    int h, grp;
+    item_head(b, key - b * (heads * p.col_groups), h, grp);
+    const int cols = min(kCols, p.rows.tokens * p.group - grp * kCols);
+    const int64_t sl = 2 * (static_cast<int64_t>(blockIdx.x) * Cfg::kTeams + w0) + 1;
+    for (int u = tid; u < cols * (D / 4); u += blockDim.x) {  // four dims of a column
+      const int col = u / (D / 4), dim = (u % (D / 4)) * 4;
       float m_shift = -INFINITY, m = -INFINITY, l = 0.f;
+      float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
       for (int w = w0; w < w1; ++w) {
-        const float4 st = stats[w * kKv8Cols + col8];
-        m_shift = fmaxf(m_shift, st.x);
-        m = fmaxf(m, st.y);
-      }
-      float v[16];
-#pragma unroll
-      for (int y = 0; y < 16; ++y) v[y] = 0.f;
-      for (int w = w0; w < w1; ++w) {
-        const float4 st = stats[w * kKv8Cols + col8];
-        const float fo = st.x == -INFINITY ? 0.f : ex2(st.x - m_shift);
-        l += st.y == -INFINITY ? st.z : st.z * ex2(st.y - m);
-        const float* src = osh + w * (D * kKv8Cols) + i * 32 * 32 + ln;
-#pragma unroll
-        for (int y = 0; y < 8; ++y) {
-          v[2 * y] += fo * src[(y * 4 + x) * 32];
-          v[2 * y + 1] += fo * src[(y * 4 + 2 + x) * 32];
-        }
+        const float2 f = join(m_shift, m, l, stats[w * kCols + col]);
+        axpby(v, f, *reinterpret_cast<const float4*>(osh + (w * kCols + col) * Cfg::kOutRow + dim));
       }
       if (whole) {
-        put(it.b, h, block, col8, i, ln >> 2, v, out_factor(m_shift, m, l));
-        if (i == 0 && (ln >> 2) == 0) put_lse(it.b, h, block, col8, m, l);
+        put_dims(p, b, h, grp * kCols + col, dim, v, out_factor(m_shift, m, l));
+        if (dim == 0) put_lse(p, b, h, grp * kCols + col, m, l);
       } else {
-        const int64_t sl = 2 * (static_cast<int64_t>(blockIdx.x) * kKv8Warps + w0) + 1;
-        float* po = p.part_o + sl * (D * kKv8Cols) + i * 32 * 32 + ln;
-        if (block * kKv8Cols + col8 < p.rows.tokens * p.group) {
-#pragma unroll
-          for (int y = 0; y < 8; ++y) {
-            po[(y * 4 + x) * 32] = v[2 * y];
-            po[(y * 4 + 2 + x) * 32] = v[2 * y + 1];
-          }
-        }
-        if (i == 0 && (ln >> 2) == 0)
-          p.part_ml[sl * kKv8Cols + col8] = make_float4(m_shift, m, l, 0.f);
+        *reinterpret_cast<float4*>(p.part_o + sl * Cfg::kOut + col * D + dim) = v;
+        if (dim == 0) p.part_ml[sl * kCols + col] = make_float4(m_shift, m, l, 0.f);
       }
     }
     w0 = w1;
   }
 }
 
-// Items that span CTAs: the sum of their parts, one CTA per (item, 128 dims).  A
-// part is the tail of the first warp of the item in each CTA, and, where the item
-// ends inside a warp's run, the head of that warp.  Four groups of threads take
-// every fourth part each; shared memory joins them in order.
-template <int D>
-__global__ void __launch_bounds__(256) kv8_merge_kernel(const Kv8AttnParams p) {
-  __shared__ float sh_o[3][64][16];
-  __shared__ float4 sh_ml[3][64];
+// Items that span CTAs: the sum of their parts.  A part is the tail of the first run
+// of the item in each CTA, and, where the item ends inside a run, that run's head.
+// A CTA takes kThreads / kSub units (four dims of a column) of one item; kSub groups
+// of threads take every kSub-th part each, kAhead of them in flight, and shared memory
+// joins them in order.  kSub = 8 when an item has many parts (few long sequences: the
+// parts are read by many threads at once), 1 when most have two or three.
+template <int kSub, int kThreads, int kAhead>
+__global__ void __launch_bounds__(kThreads) kv8_merge_kernel(const Kv8AttnParams p, const int d,
+                                                        const int teams) {
+  constexpr int kUnits = kThreads / kSub;
+  __shared__ float4 sh_o[kSub][kUnits];
+  __shared__ float4 sh_ml[kSub][kUnits];
   pdl_enter();
-  const int items = p.cache.heads * p.col_blocks;
+  const int B = p.rows.batch, items = p.cache.heads * p.col_groups;
   const int b = blockIdx.x / items, rest = blockIdx.x % items;
-  const int h = rest / p.col_blocks, block = rest % p.col_blocks;
-  const Kv8Row row = kv8_row(p.cache, p.rows, b, p.max_k);
-  RowPlan r;
-  r.slot = row.slot;
-  r.start = row.start;
-  r.n = row.n;
-  r.lo = p.window > 0 ? max(0, row.start - p.window + 1) : 0;
-  const int act = active_blocks(r, p.group);
-  if (block >= act) return;  // padding: written by the warp that met it
-  const int per = p.plan[0];
+  const int h = rest / p.col_groups, grp = rest % p.col_groups;
+  const int4 head4 = *reinterpret_cast<const int4*>(p.plan);
+  const int4 row4 = reinterpret_cast<const int4*>(p.plan)[1 + b];
+  const int row_first = p.plan[4 + 4 * B + b];
+  const int runs = head4.x, total = head4.y;
+  const RowPlan r = {row4.x, row4.y, row4.z, row4.w};
+  const int act = (r.n * p.group + p.cols - 1) / p.cols;
+  if (grp >= act) return;  // padding: written by the run that met it
   const int nt = row_tiles(r);
-  const int i0 = p.plan[1 + b] + (h * act + block) * nt, i1 = i0 + nt;
-  const int w0 = i0 / per, w1 = (i1 - 1) / per;
-  if (w0 == w1) return;  // one warp had it all
-  const int total = p.plan[1 + p.rows.batch];
-  const bool has_head = i1 < min(total, (w1 + 1) * per);      // ends inside warp w1's run
-  if (!has_head && w0 / kKv8Warps == w1 / kKv8Warps) return;  // one CTA had it all
+  const int i0 = row_first + (h * act + grp) * nt, i1 = i0 + nt;
+  const int w0 = run_of(i0, runs, total), w1 = run_of(i1 - 1, runs, total);
+  if (w0 == w1) return;                                       // one run had it all
+  const bool has_head = i1 < run_begin(w1 + 1, runs, total);  // ends inside run w1
+  if (!has_head && w0 / teams == w1 / teams) return;          // one CTA had it all
   // CTAs that hold a tail of it
-  const int c0 = w0 / kKv8Warps, c1 = (has_head ? w1 - 1 : w1) / kKv8Warps;
+  const int c0 = w0 / teams, c1 = (has_head ? w1 - 1 : w1) / teams;
   const int parts = c1 - c0 + 1 + (has_head ? 1 : 0);
-  const int tid = threadIdx.x, sub = tid >> 6, u = tid & 63;
-  const int ln = u & 31, x = u >> 5, i = blockIdx.y;
-  const int col8 = 2 * (ln & 3) + x;
-  const bool col_ok = block * kKv8Cols + col8 < p.rows.tokens * p.group;
-  float m_shift = -INFINITY, m = -INFINITY, l = 0.f, v[16];
+  const int sub = threadIdx.x / kUnits, u = threadIdx.x % kUnits;
+  const int unit = blockIdx.y * kUnits + u, quads = d / 4;
+  const int col = unit / quads, dim = (unit % quads) * 4;
+  const bool ok = col < min(p.cols, p.rows.tokens * p.group - grp * p.cols);
+  const int64_t out = static_cast<int64_t>(p.cols) * d;
+  float m_shift = -INFINITY, m = -INFINITY, l = 0.f;
+  float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (ok) {
+    for (int k0 = sub; k0 < parts; k0 += kAhead * kSub) {
+      float4 o[kAhead], st[kAhead];
 #pragma unroll
-  for (int y = 0; y < 16; ++y) v[y] = 0.f;
-  if (col_ok) {
-    for (int k = sub; k < parts; k += 4) {
-      const int c = c0 + k;
-      const int64_t sl = c <= c1 ? 2 * static_cast<int64_t>(max(w0, c * kKv8Warps)) + 1
-                                 : 2 * static_cast<int64_t>(w1);
-      const float4 st = p.part_ml[sl * kKv8Cols + col8];
-      const float* po = p.part_o + sl * (D * kKv8Cols) + i * 32 * 32 + ln;
-      float o[16];
-#pragma unroll
-      for (int y = 0; y < 8; ++y) {
-        o[2 * y] = po[(y * 4 + x) * 32];
-        o[2 * y + 1] = po[(y * 4 + 2 + x) * 32];
+      for (int j = 0; j < kAhead; ++j) {
+        const int k = k0 + j * kSub;
+        if (k < parts) {
+          const int c = c0 + k;
+          const int64_t sl = c <= c1 ? 2 * static_cast<int64_t>(max(w0, c * teams)) + 1
+                                     : 2 * static_cast<int64_t>(w1);
+          st[j] = p.part_ml[sl * p.cols + col];
+          o[j] = *reinterpret_cast<const float4*>(p.part_o + sl * out + col * d + dim);
+        }
       }
-      const float ms = fmaxf(m_shift, st.x), mn = fmaxf(m, st.y);
-      const float fa = m_shift == -INFINITY ? 0.f : ex2(m_shift - ms);
-      const float fb = st.x == -INFINITY ? 0.f : ex2(st.x - ms);
-      l = (m == -INFINITY ? l : l * ex2(m - mn)) + (st.y == -INFINITY ? st.z : st.z * ex2(st.y - mn));
 #pragma unroll
-      for (int y = 0; y < 16; ++y) v[y] = v[y] * fa + o[y] * fb;
-      m_shift = ms;
-      m = mn;
+      for (int j = 0; j < kAhead; ++j)
+        if (k0 + j * kSub < parts) axpby(v, join(m_shift, m, l, st[j]), o[j]);
     }
   }
-  if (sub > 0) {
-#pragma unroll
-    for (int y = 0; y < 16; ++y) sh_o[sub - 1][u][y] = v[y];
-    sh_ml[sub - 1][u] = make_float4(m_shift, m, l, 0.f);
+  if constexpr (kSub > 1) {
+    sh_o[sub][u] = v;
+    sh_ml[sub][u] = make_float4(m_shift, m, l, 0.f);
+    __syncthreads();
+    if (sub > 0) return;
+    for (int k = 1; k < kSub; ++k) axpby(v, join(m_shift, m, l, sh_ml[k][u]), sh_o[k][u]);
   }
-  __syncthreads();
-  if (sub > 0 || !col_ok) return;
-#pragma unroll 1
-  for (int k = 0; k < 3; ++k) {
-    const float4 st = sh_ml[k][u];
-    const float ms = fmaxf(m_shift, st.x), mn = fmaxf(m, st.y);
-    const float fa = m_shift == -INFINITY ? 0.f : ex2(m_shift - ms);
-    const float fb = st.x == -INFINITY ? 0.f : ex2(st.x - ms);
-    l = (m == -INFINITY ? l : l * ex2(m - mn)) + (st.y == -INFINITY ? st.z : st.z * ex2(st.y - mn));
-#pragma unroll
-    for (int y = 0; y < 16; ++y) v[y] = v[y] * fa + sh_o[k][u][y] * fb;
-    m_shift = ms;
-    m = mn;
-  }
-  const float f = l == 0.f || m_shift == -INFINITY ? 0.f : ex2(m_shift - kShiftUp - m) / l;
-  const int col = block * kKv8Cols + col8;
-  const int tok = col / p.group, qh = h * p.group + col - tok * p.group;
-  uint32_t w[8];
-#pragma unroll
-  for (int y = 0; y < 8; ++y) w[y] = pack_bf16x2(v[2 * y] * f, v[2 * y + 1] * f);
-  uint4* dst = reinterpret_cast<uint4*>(p.o + static_cast<int64_t>(b) * p.o_stride[0] +
-                                        static_cast<int64_t>(tok) * p.o_stride[1] +
-                                        static_cast<int64_t>(qh) * p.o_stride[2] +
-                                        v_chunk(ln >> 2, i) * 16);
-  dst[0] = make_uint4(w[0], w[1], w[2], w[3]);
-  dst[1] = make_uint4(w[4], w[5], w[6], w[7]);
-  if (i == 0 && (ln >> 2) == 0)
-    p.lse[static_cast<int64_t>(b) * p.lse_stride[0] + static_cast<int64_t>(qh) * p.lse_stride[1] +
-          tok] = l > 0.f ? (m + __log2f(l)) * kLn2 : (l == 0.f ? -INFINITY : l);
+  if (!ok) return;
+  put_dims(p, b, h, grp * p.cols + col, dim, v, out_factor(m_shift, m, l));
+  if (dim == 0) put_lse(p, b, h, grp * p.cols + col, m, l);
 }
 
 namespace {
-template <int D, bool kInt8>
+
+// The launch shapes.  One block of 8 columns (decode): 256 dims per warp, 12 warps
+// (170 registers).  More columns: three blocks at once and 128 dims per warp, 8
+// warps (255 registers).
+template <int D>
+using OneBlock = AttnShape<D, D / 256, 1, 12, 3>;
+template <int D>
+using ThreeBlocks = AttnShape<D, D / 128, 3, 8, 8>;
+
+template <typename Cfg, bool kInt8>
 int launch_attn(const Kv8AttnParams& p, int ctas, cudaStream_t stream) {
-  const int smem = AttnCfg<D>::smem(p.rows.batch);
-  cudaError_t e = cudaFuncSetAttribute(kv8_attn_kernel<D, kInt8>,
+  const int smem = Cfg::smem(p.rows.batch);
+  cudaError_t e = cudaFuncSetAttribute(kv8_attn_kernel<Cfg, kInt8>,
                                        cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e == cudaSuccess)
-    e = launch_chained(kv8_attn_kernel<D, kInt8>, dim3(ctas), dim3(kKv8Warps * 32), smem, stream,
+    e = launch_chained(kv8_attn_kernel<Cfg, kInt8>, dim3(ctas), dim3(Cfg::kThreads), smem, stream,
                        p);
   return static_cast<int>(e);
 }
-}  // namespace
-
-int launch_kv8_attn(int d, bool int8, const Kv8AttnParams& p, int ctas, cudaStream_t stream) {
-  if (d == 512) return int8 ? launch_attn<512, true>(p, ctas, stream)
-                            : launch_attn<512, false>(p, ctas, stream);
-  return int8 ? launch_attn<256, true>(p, ctas, stream) : launch_attn<256, false>(p, ctas, stream);
+template <typename Cfg>
+Kv8AttnShape shape_of() {
+  return {Cfg::kCols, Cfg::kTeams, Cfg::kOut};
 }
 
-int launch_kv8_merge(int d, const Kv8AttnParams& p, cudaStream_t stream) {
-  const dim3 grid(p.rows.batch * p.cache.heads * p.col_blocks, d / 128);
-  return static_cast<int>(
-      d == 512 ? launch_chained(kv8_merge_kernel<512>, grid, dim3(256), 0, stream, p)
-               : launch_chained(kv8_merge_kernel<256>, grid, dim3(256), 0, stream, p));
+}  // namespace
+
+Kv8AttnShape kv8_attn_shape(int d, int64_t columns) {
+  if (columns <= 8) return d == 512 ? shape_of<OneBlock<512>>() : shape_of<OneBlock<256>>();
+  return d == 512 ? shape_of<ThreeBlocks<512>>() : shape_of<ThreeBlocks<256>>();
+}
+
+int launch_kv8_attn(int d, bool int8, const Kv8AttnParams& p, int ctas, cudaStream_t stream) {
+  if (p.cols == 8) {
+    if (d == 512) return int8 ? launch_attn<OneBlock<512>, true>(p, ctas, stream)
+                              : launch_attn<OneBlock<512>, false>(p, ctas, stream);
+    return int8 ? launch_attn<OneBlock<256>, true>(p, ctas, stream)
+                : launch_attn<OneBlock<256>, false>(p, ctas, stream);
+  }
+  if (d == 512) return int8 ? launch_attn<ThreeBlocks<512>, true>(p, ctas, stream)
+                            : launch_attn<ThreeBlocks<512>, false>(p, ctas, stream);
+  return int8 ? launch_attn<ThreeBlocks<256>, true>(p, ctas, stream)
+              : launch_attn<ThreeBlocks<256>, false>(p, ctas, stream);
+}
+
+int launch_kv8_merge(int d, const Kv8AttnParams& p, int ctas, cudaStream_t stream) {
+  const int teams = kv8_attn_shape(d, p.cols).runs;
+  const int items = p.rows.batch * p.cache.heads * p.col_groups;
+  const int columns = std::min(p.cols, p.rows.tokens * p.group);
+  const int units = columns * (d / 4);
+  // parts per item: about one per CTA that it spans
+  if (ctas >= 8 * items)
+    return static_cast<int>(launch_chained(kv8_merge_kernel<8, 256, 8>,
+                                           dim3(items, (units + 31) / 32), dim3(256), 0, stream, p,
+                                           d, teams));
+  return static_cast<int>(launch_chained(kv8_merge_kernel<1, 128, 2>,
+                                         dim3(items, (units + 127) / 128), dim3(128), 0, stream, p,
+                                         d, teams));
 }
 
 }  // namespace g4

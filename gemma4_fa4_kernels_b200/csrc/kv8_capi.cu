@@ -14,6 +14,22 @@ namespace {
 
 using namespace g4;
 
+// Makes the call's device current while it launches, and the caller's again after.
+class OnDevice {
+ public:
+  explicit OnDevice(int device) {
+    if (device >= 0 && cudaGetDevice(&before_) == cudaSuccess && before_ != device)
+      moved_ = cudaSetDevice(device) == cudaSuccess;
+  }
+  ~OnDevice() {
+    if (moved_) cudaSetDevice(before_);
+  }
+
+ private:
+  int before_ = 0;
+  bool moved_ = false;
+};
+
 bool al16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 size_t up256(size_t x) { return (x + 255) & ~static_cast<size_t>(255); }
 
@@ -96,31 +112,33 @@ int check_attn_shape(const g4_kv8_args* a) {
 // Launch shape and workspace of the attention.
 struct AttnPlan {
   int64_t tiles = 0;  // upper bound of the tile list
-  int col_blocks = 0;
+  int cols = 0, col_groups = 0;
   int ctas = 0;
   size_t part_o = 0, part_ml = 0, plan = 0, total = 0;
 };
 
 AttnPlan attn_plan(const g4_kv8_args* a) {
   AttnPlan w;
-  const int64_t group = a->num_q_heads / a->num_kv_heads;
-  const int64_t cols = group * a->tokens;
-  w.col_blocks = static_cast<int>(std::min<int64_t>((cols + kKv8Cols - 1) / kKv8Cols, INT32_MAX));
+  const int64_t columns = int64_t(a->num_q_heads / a->num_kv_heads) * a->tokens;
+  const Kv8AttnShape shape = kv8_attn_shape(a->head_dim, columns);
+  w.cols = shape.cols;
+  w.col_groups = static_cast<int>(
+      std::min<int64_t>((columns + shape.cols - 1) / shape.cols, INT32_MAX));
   int64_t keys = a->max_seqlen_k;
   if (a->window > 0) keys = std::min<int64_t>(keys, int64_t(a->window) + a->tokens - 1);
   const int64_t per_item = (keys + kKv8Tile - 1) / kKv8Tile + 1;
-  w.tiles = int64_t(a->batch) * a->num_kv_heads * w.col_blocks * per_item;
-  // one CTA per SM; fewer when there is less than a tile per warp
-  w.ctas = static_cast<int>(
-      std::max<int64_t>(1, std::min<int64_t>(api_sm_count(), (w.tiles + kKv8Warps - 1) / kKv8Warps)));
-  const size_t slots = size_t(w.ctas) * kKv8Warps * 2;
+  w.tiles = int64_t(a->batch) * a->num_kv_heads * w.col_groups * per_item;
+  // one CTA per SM; fewer when there is less than a tile per run
+  w.ctas = static_cast<int>(std::max<int64_t>(
+      1, std::min<int64_t>(api_sm_count(), (w.tiles + shape.runs - 1) / shape.runs)));
+  const size_t slots = size_t(w.ctas) * shape.runs * 2;
   size_t off = 0;
   w.plan = off;
-  off = up256(off + sizeof(int) * (size_t(a->batch) + 2));
+  off = up256(off + sizeof(int) * (5 * size_t(a->batch) + 4));
   w.part_ml = off;
-  off = up256(off + slots * kKv8Cols * sizeof(float4));
+  off = up256(off + slots * shape.cols * sizeof(float4));
   w.part_o = off;
-  off = up256(off + slots * kKv8Cols * size_t(a->head_dim) * sizeof(float));
+  off = up256(off + slots * size_t(shape.out_floats) * sizeof(float));
   w.total = off;
   return w;
 }
@@ -231,6 +249,7 @@ int g4_kv8_append(const g4_kv8_args* a, void* stream) {
     p.v_stride[i] = a->v_stride[i];
   }
   p.status = a->status;
+  const OnDevice guard(a->device);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   LaunchScope ls(kKKv8Append, st);
   return launched(launch_kv8_append(a->head_dim, a->format == G4_KV8_INT8, p, st),
@@ -257,6 +276,7 @@ int g4_kv8_read(const g4_kv8_args* a, void* stream) {
   for (int i = 0; i < 3; ++i) p.out_stride[i] = a->k_stride[i];
   p.out_rows = a->out_rows;
   p.out_total = a->out_total;
+  const OnDevice guard(a->device);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   LaunchScope ls(kKKv8Read, st);
   return launched(launch_kv8_read(a->head_dim, a->format == G4_KV8_INT8, p, st),
@@ -268,6 +288,7 @@ size_t g4_kv8_attn_workspace_bytes(const g4_kv8_args* a) {
     api_clear_error();
     return 0;
   }
+  const OnDevice guard(a->device);
   return attn_plan(a).total;
 }
 
@@ -280,8 +301,9 @@ int g4_kv8_attn(const g4_kv8_args* a, void* stream) {
   if ((rc = check_operand(a->o, a->o_stride, "o", true))) return rc;
   if (!a->lse || a->lse_stride[0] <= 0 || a->lse_stride[1] <= 0)
     return api_fail(G4_ERR_INVALID, "lse with positive strides is required");
+  const OnDevice guard(a->device);
   const AttnPlan w = attn_plan(a);
-  // the list index and its products with the warp number stay below 2^31
+  // list indices stay below 2^31
   if (w.tiles > (int64_t(1) << 30))
     return api_fail(G4_ERR_UNSUPPORTED, "too many (row, head, token, key) tiles in one call");
   if (!a->workspace || !al16(a->workspace) || a->workspace_bytes < w.total)
@@ -294,7 +316,8 @@ int g4_kv8_attn(const g4_kv8_args* a, void* stream) {
   p.window = a->window;
   p.max_k = a->max_seqlen_k;
   p.group = a->num_q_heads / a->num_kv_heads;
-  p.col_blocks = w.col_blocks;
+  p.cols = w.cols;
+  p.col_groups = w.col_groups;
   p.q = static_cast<const __nv_bfloat16*>(a->q);
   p.o = static_cast<__nv_bfloat16*>(a->o);
   for (int i = 0; i < 3; ++i) {
@@ -316,7 +339,7 @@ int g4_kv8_attn(const g4_kv8_args* a, void* stream) {
   }
   if (w.ctas > 1) {  // one CTA sums its own parts
     LaunchScope ls(kKKv8Merge, st);
-    return launched(launch_kv8_merge(a->head_dim, p, st), "cache attention merge launch");
+    return launched(launch_kv8_merge(a->head_dim, p, w.ctas, st), "cache attention merge launch");
   }
   return G4_OK;
 }
@@ -343,6 +366,7 @@ int g4_kv8_chunk_plan(const g4_kv8_args* a, int32_t* cu_q, int32_t* cu_k, int32_
   p.cu_k = cu_k;
   p.first = first;
   p.last = last;
+  const OnDevice guard(a->device);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   LaunchScope ls(kKKv8Chunk, st);
   return launched(launch_kv8_chunk_plan(p, st), "chunk plan launch");
@@ -356,6 +380,7 @@ int g4_kv8_pad_rows(const g4_kv8_args* a, void* stream) {
   if ((rc = check_operand(a->o, a->o_stride, "o", true))) return rc;
   if (!a->lse || a->lse_stride[0] <= 0 || a->lse_stride[1] <= 0)
     return api_fail(G4_ERR_INVALID, "lse with positive strides is required");
+  const OnDevice guard(a->device);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   LaunchScope ls(kKKv8Chunk, st);
   return launched(launch_kv8_pad_rows(cache_of(a), rows_of(a), a->max_seqlen_k, a->num_q_heads,
@@ -373,6 +398,7 @@ int g4_pages_extend(const g4_pages_args* a, void* stream) {
   if ((rc = check_batch(a, true))) return rc;
   if (!a->first || !a->counts || !a->starts || !a->ends)
     return api_fail(G4_ERR_INVALID, "slots, counts, starts and ends are required");
+  const OnDevice guard(a->device);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   LaunchScope ls(kKPagesPlan, st);
   return launched(launch_pages_extend(pages_of(a), st), "page reservation launch");
@@ -388,6 +414,7 @@ int g4_pages_fork(const g4_pages_args* a, void* stream) {
     return api_fail(G4_ERR_INVALID, "parents and children are required");
   if ((rc = check_work(a, up256(sizeof(int) * 3 * size_t(a->batch))))) return rc;
   const Kv8PagesParams p = pages_of(a);
+  const OnDevice guard(a->device);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   {
     LaunchScope ls(kKPagesPlan, st);
@@ -406,6 +433,7 @@ int g4_pages_free(const g4_pages_args* a, void* stream) {
   if ((rc = check_batch(a, true))) return rc;
   if (!a->first) return api_fail(G4_ERR_INVALID, "slots are required");
   if (a->window < 0) return api_fail(G4_ERR_INVALID, "window must be >= 0");
+  const OnDevice guard(a->device);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   LaunchScope ls(kKPagesPlan, st);
   return launched(launch_pages_free(pages_of(a), st), "page release launch");
@@ -418,6 +446,7 @@ int g4_pages_compact(const g4_pages_args* a, void* stream) {
   if ((rc = check_pools(a))) return rc;
   if ((rc = check_work(a, up256(sizeof(int) * (2 + 3 * size_t(a->num_pages)))))) return rc;
   const Kv8PagesParams p = pages_of(a);
+  const OnDevice guard(a->device);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   {
     LaunchScope ls(kKPagesPlan, st);
@@ -437,6 +466,7 @@ int g4_pages_copy(const g4_pages_args* a, void* stream) {
   if (!a->first || !a->second)
     return api_fail(G4_ERR_INVALID, "source and destination pages are required");
   const Kv8PagesParams p = pages_of(a);
+  const OnDevice guard(a->device);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   LaunchScope ls(kKPagesApply, st);
   const int64_t units = 2 * int64_t(p.layers) * ((p.page_bytes + 16383) / 16384);

@@ -56,18 +56,6 @@ MAX_ROWS = 1024
 DIRECT_COLUMNS = 128
 
 
-def _ints(t, rows: int | None, name: str, device) -> torch.Tensor:
-    if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.dim() != 1:
-        raise ValueError(f"{name} must be a one-dimensional int32 tensor")
-    if rows is not None and t.shape[0] != rows:
-        raise ValueError(f"{name} must have {rows} entries, found {t.shape[0]}")
-    if t.device != device:
-        raise ValueError(f"{name} must be on the cache's device ({device})")
-    if not t.is_contiguous():
-        raise ValueError(f"{name} must be contiguous")
-    return t
-
-
 def _strides(t: torch.Tensor) -> list[int]:
     """(batch, token, head) strides; a dimension of size one has none that matter."""
     return [t.shape[-1] if n == 1 else s for n, s in zip(t.shape[:3], t.stride()[:3])]
@@ -133,29 +121,23 @@ class PagedKVCache8:
         self.num_layers, self.num_pages, self.num_kv_heads, self.page_size, self.head_dim = k.shape
         self.max_slots, self.pages_per_slot = tables.shape
         self.capacity = self.pages_per_slot * self.page_size  # tokens a slot can hold
-        self._blocks: dict = {}
+        self._calls: dict = {}
 
     # ----------------------------------------------------------------------------
     # arguments
     # ----------------------------------------------------------------------------
+    # What a call checks and lays out depends on its operands' shapes, strides and
+    # types only.  It is done once per signature and kept as a finished argument
+    # block; a call copies the block and writes its pointers (a decode step of a
+    # small batch is otherwise bound by this host work).
     def _on_device(self) -> None:
         if self.device.type != "cuda":
             raise UnsupportedB200Path("the paged cache's operators require a CUDA device")
 
     def _launch(self, fn, *args) -> None:
-        """``fn(*args, stream)`` on the cache's device; the status as an exception."""
-        if torch.cuda.current_device() == self.device.index:
-            rc = fn(*args, _stream(self.device))
-        else:
-            with torch.cuda.device(self.device):
-                rc = fn(*args, _stream(self.device))
+        rc = fn(*args, _stream(self.device))
         if rc:
             _raise_for(rc, fn.__name__)
-
-    def _layer(self, layer: int) -> int:
-        if not 0 <= layer < self.num_layers:
-            raise IndexError(f"layer {layer} of a cache of {self.num_layers}")
-        return layer
 
     def _operand(self, t: torch.Tensor, heads: int | None, name: str) -> None:
         if t.dim() != 4 or t.dtype != torch.bfloat16:
@@ -165,48 +147,66 @@ class PagedKVCache8:
                              f"({self.num_kv_heads} KV heads, head_dim {self.head_dim})")
         if t.device != self.device:
             raise ValueError(f"{name} must be on the cache's device ({self.device})")
-        if t.shape[3] > 1 and t.stride(3) != 1:
+        if t.stride(3) != 1:
             raise ValueError(f"{name} must have unit stride along head_dim")
-        if t.requires_grad and torch.is_grad_enabled():
-            raise UnsupportedB200Path(f"the paged cache is inference only: {name} requires grad")
-
-    def _rows(self, a, batch: int, slots, starts, ends) -> None:
-        if slots is None:
-            if batch > self.max_slots:
-                raise ValueError("more rows than slots")
-        else:
-            a.slots = _ints(slots, batch, "slots", self.device).data_ptr()
-        a.starts = _ints(starts, batch, "starts", self.device).data_ptr()
-        a.ends = _ints(ends, batch, "ends", self.device).data_ptr()
-
-    def _check_rows(self, batch: int, tokens: int) -> None:
-        if batch > MAX_ROWS:
+        if t.shape[0] > MAX_ROWS:
             raise UnsupportedB200Path(f"at most {MAX_ROWS} rows per call")
 
-    def _kv8(self, key, layer: int, batch: int, tokens: int, fill) -> _lib.G4Kv8Args:
-        """The argument block of a call signature (a copy of a cached one): all
-        but the pointers of the call's own tensors."""
-        key = (layer, batch, tokens, *key)
-        block = self._blocks.get(key)
-        if block is None:
-            a = _lib.G4Kv8Args()
-            a.k_pages, a.v_pages = self.k[layer].data_ptr(), self.v[layer].data_ptr()
-            a.k_scale, a.v_scale = self.k_scale[layer].data_ptr(), self.v_scale[layer].data_ptr()
-            a.tables, a.status = self.tables.data_ptr(), self.status.data_ptr()
-            a.format = CODE_DTYPES[self.k.dtype]
-            a.num_pages, a.page_size = self.num_pages, self.page_size
-            a.num_kv_heads, a.head_dim = self.num_kv_heads, self.head_dim
-            a.num_slots, a.pages_per_slot = self.max_slots, self.pages_per_slot
-            a.batch, a.tokens = batch, tokens
-            fill(a)
-            if len(self._blocks) >= 512:
-                self._blocks.clear()
-            self._blocks[key] = block = bytes(a)
-        return _lib.G4Kv8Args.from_buffer_copy(block)
+    @staticmethod
+    def _no_grad(*tensors) -> None:
+        if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+            raise UnsupportedB200Path("the paged cache is inference only: an operand requires grad")
+
+    def _ints(self, t, rows: int | None, name: str) -> torch.Tensor:
+        """``t``, a contiguous int32 vector of ``rows`` entries on the cache's device."""
+        if (isinstance(t, torch.Tensor) and t.dtype is torch.int32 and t.dim() == 1
+                and t.device == self.device and t.is_contiguous()
+                and (rows is None or t.shape[0] == rows)):
+            return t
+        if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.dim() != 1:
+            raise ValueError(f"{name} must be a one-dimensional int32 tensor")
+        if t.device != self.device:
+            raise ValueError(f"{name} must be on the cache's device ({self.device})")
+        if not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous")
+        raise ValueError(f"{name} must have {rows} entries, found {t.shape[0]}")
+
+    def _rows(self, a, batch: int, slots, starts, ends) -> None:
+        if slots is not None:
+            a.slots = self._ints(slots, batch, "slots").data_ptr()
+        elif batch > self.max_slots:
+            raise ValueError("more rows than slots")
+        a.starts = self._ints(starts, batch, "starts").data_ptr()
+        a.ends = self._ints(ends, batch, "ends").data_ptr()
+        if self.device.type != "cuda":
+            self._on_device()
+
+    def _block(self, layer: int, batch: int, tokens: int) -> _lib.G4Kv8Args:
+        """A new argument block of one layer's cache."""
+        if not 0 <= layer < self.num_layers:
+            raise IndexError(f"layer {layer} of a cache of {self.num_layers}")
+        a = _lib.G4Kv8Args()
+        a.k_pages, a.v_pages = self.k[layer].data_ptr(), self.v[layer].data_ptr()
+        a.k_scale, a.v_scale = self.k_scale[layer].data_ptr(), self.v_scale[layer].data_ptr()
+        a.tables, a.status = self.tables.data_ptr(), self.status.data_ptr()
+        a.format = CODE_DTYPES[self.k.dtype]
+        a.num_pages, a.page_size = self.num_pages, self.page_size
+        a.num_kv_heads, a.head_dim = self.num_kv_heads, self.head_dim
+        a.num_slots, a.pages_per_slot = self.max_slots, self.pages_per_slot
+        a.batch, a.tokens = batch, tokens
+        a.device = -1 if self.device.index is None else self.device.index
+        return a
+
+    def _keep(self, key, call):
+        if len(self._calls) >= 512:
+            self._calls.clear()
+        self._calls[key] = call
+        return call
 
     def _pages(self, batch: int, first=None, second=None, workspace=False):
-        block = self._blocks.get("pages")
+        block = self._calls.get("pages")
         if block is None:
+            self._on_device()
             a = _lib.G4PagesArgs()
             a.tables, a.lengths = self.tables.data_ptr(), self.lengths.data_ptr()
             a.refcounts, a.status = self.refcounts.data_ptr(), self.status.data_ptr()
@@ -215,7 +215,8 @@ class PagedKVCache8:
             a.num_layers, a.num_pages, a.page_size = self.num_layers, self.num_pages, self.page_size
             a.num_kv_heads, a.head_dim = self.num_kv_heads, self.head_dim
             a.num_slots, a.pages_per_slot = self.max_slots, self.pages_per_slot
-            self._blocks["pages"] = block = bytes(a)
+            a.device = -1 if self.device.index is None else self.device.index
+            block = self._keep("pages", bytes(a))
         a = _lib.G4PagesArgs.from_buffer_copy(block)
         a.batch = batch
         if first is not None:
@@ -235,49 +236,56 @@ class PagedKVCache8:
         """Quantise ``k`` and ``v`` (rows, tokens, KV heads, head_dim) BF16 and write
         each row's first ``ends - starts`` tokens at its positions, whose pages the
         tables must list (:meth:`extend`).  ``slots`` None: row b is slot b."""
-        self._layer(layer)
+        key = ("append", layer, k.shape, k.stride(), k.dtype, k.device, v.shape, v.stride(),
+               v.dtype, v.device)
+        call = self._calls.get(key) or self._append_call(key, layer, k, v)
+        self._no_grad(k, v)
+        batch, block = call
+        if block is None:
+            return
+        a = _lib.G4Kv8Args.from_buffer_copy(block)
+        self._rows(a, batch, slots, starts, ends)
+        a.k, a.v = k.data_ptr(), v.data_ptr()
+        self._launch(_lib.load().g4_kv8_append, ctypes.byref(a))
+
+    def _append_call(self, key, layer, k, v):
         self._operand(k, self.num_kv_heads, "k")
         self._operand(v, self.num_kv_heads, "v")
         if v.shape != k.shape:
             raise ValueError("k and v must have one shape")
         batch, tokens = k.shape[:2]
-        self._check_rows(batch, tokens)
-        ks, vs = _strides(k), _strides(v)
-
-        def fill(a):
-            a.k_stride[:], a.v_stride[:] = ks, vs
-
-        if batch == 0 or tokens == 0:
-            return
-        a = self._kv8(("append", *ks, *vs), layer, batch, tokens, fill)
-        self._rows(a, batch, slots, starts, ends)
-        self._on_device()
-        a.k, a.v = k.data_ptr(), v.data_ptr()
-        self._launch(_lib.load().g4_kv8_append, ctypes.byref(a))
+        a = self._block(layer, batch, tokens)
+        a.k_stride[:], a.v_stride[:] = _strides(k), _strides(v)
+        return self._keep(key, (batch, bytes(a) if batch and tokens else None))
 
     def read(self, layer: int, slots, starts, ends, max_tokens: int):
         """Values at positions ``starts .. ends - 1`` of each row: K and V, BF16
         (rows, max_tokens, KV heads, head_dim), zeros past a row's end and where it
         has no page.  Exact for what :meth:`append` wrote."""
-        self._layer(layer)
-        batch = _ints(starts, None, "starts", self.device).shape[0]
+        batch = self._ints(starts, None, "starts").shape[0]
+        if batch > MAX_ROWS:
+            raise UnsupportedB200Path(f"at most {MAX_ROWS} rows per call")
         if max_tokens < 0:
             raise ValueError("max_tokens must be >= 0")
-        self._check_rows(batch, max_tokens)
         shape = (batch, max_tokens, self.num_kv_heads, self.head_dim)
         k = torch.empty(shape, dtype=torch.bfloat16, device=self.device)
-        v = torch.empty(shape, dtype=torch.bfloat16, device=self.device)
-        if k.numel():
-            self._read(layer, slots, starts, ends, k, v, _strides(k), batch, max_tokens, None)
+        v = torch.empty_like(k)
+        if batch and max_tokens:
+            self._read(layer, slots, starts, ends, k, v, batch, max_tokens, None)
+        elif not 0 <= layer < self.num_layers:
+            raise IndexError(f"layer {layer} of a cache of {self.num_layers}")
         return k, v
 
-    def _read(self, layer, slots, starts, ends, k, v, strides, batch, tokens, out_rows) -> None:
-        def fill(a):
-            a.k_stride[:] = a.v_stride[:] = strides
-
-        a = self._kv8(("read", *strides), layer, batch, tokens, fill)
+    def _read(self, layer, slots, starts, ends, k, v, batch, tokens, out_rows) -> None:
+        key = ("read", layer, batch, tokens, out_rows is None)
+        block = self._calls.get(key)
+        if block is None:
+            a = self._block(layer, batch, tokens)
+            row = self.num_kv_heads * self.head_dim
+            a.k_stride[:] = a.v_stride[:] = (tokens * row, row, self.head_dim)
+            block = self._keep(key, bytes(a))
+        a = _lib.G4Kv8Args.from_buffer_copy(block)
         self._rows(a, batch, slots, starts, ends)
-        self._on_device()
         a.k, a.v = k.data_ptr(), v.data_ptr()
         if out_rows is not None:
             a.out_rows, a.out_total = out_rows.data_ptr(), k.shape[0]
@@ -297,7 +305,26 @@ class PagedKVCache8:
         ``max_seqlen_k`` (default: a slot's capacity) bounds ``ends``; a tighter bound
         sizes the launch and its buffers better, and a row beyond it counts as empty.
         """
-        self._layer(layer)
+        key = ("attention", layer, window, max_seqlen_k, q.shape, q.stride(), q.dtype, q.device)
+        call = self._calls.get(key) or self._attention_call(key, layer, q, window, max_seqlen_k)
+        self._no_grad(q)
+        batch, block, lse_shape, ws_bytes, chunk = call
+        if block is None:
+            return (torch.empty(q.shape, dtype=torch.bfloat16, device=self.device),
+                    torch.empty(lse_shape, dtype=torch.float32, device=self.device))
+        a = _lib.G4Kv8Args.from_buffer_copy(block)
+        self._rows(a, batch, slots, starts, ends)
+        out = torch.empty(q.shape, dtype=torch.bfloat16, device=self.device)
+        a.o = out.data_ptr()
+        if chunk:
+            return out, self._chunk(a, layer, q, out, slots)
+        lse = torch.empty(lse_shape, dtype=torch.float32, device=self.device)
+        ws = torch.empty(ws_bytes, dtype=torch.uint8, device=self.device)
+        a.q, a.lse, a.workspace = q.data_ptr(), lse.data_ptr(), ws.data_ptr()
+        self._launch(_lib.load().g4_kv8_attn, ctypes.byref(a))
+        return out, lse
+
+    def _attention_call(self, key, layer, q, window, max_seqlen_k):
         self._operand(q, None, "q")
         batch, tokens, heads, d = q.shape
         if heads == 0 or heads % self.num_kv_heads:
@@ -305,74 +332,51 @@ class PagedKVCache8:
         if window < 0:
             raise ValueError("window must be >= 0")
         max_k = self.capacity if max_seqlen_k is None else int(max_seqlen_k)
-        if not 1 <= max_k:
+        if max_k < 1:
             raise ValueError("max_seqlen_k must be positive")
-        max_k = min(max_k, self.capacity)
-        self._check_rows(batch, tokens)
-        if batch == 0 or tokens == 0:
-            return (torch.empty_like(q, memory_format=torch.contiguous_format),
-                    q.new_empty((batch, heads, tokens), dtype=torch.float32))
-        if tokens * (heads // self.num_kv_heads) > DIRECT_COLUMNS:
-            return self._chunk(layer, q, slots, starts, ends, int(window), max_k)
-        qs = _strides(q)
-        sizes = (heads * tokens * d, heads * d, d), (heads * tokens, tokens)
+        a = self._block(layer, batch, tokens)
+        a.num_q_heads, a.window, a.max_seqlen_k = heads, int(window), min(max_k, self.capacity)
+        a.q_stride[:] = _strides(q)
+        a.o_stride[:] = (heads * tokens * d, heads * d, d)
+        if any(s <= 0 or s % 8 for s in a.q_stride):
+            raise ValueError("q strides must be positive multiples of 8 elements")
+        if not batch or not tokens:
+            return self._keep(key, (batch, None, (batch, heads, tokens), 0, False))
+        chunk = tokens * (heads // self.num_kv_heads) > DIRECT_COLUMNS
+        if chunk:  # LSE as the packed forward writes it: (head, row, token)
+            a.lse_stride[:] = (tokens, batch * tokens)
+            ws_bytes = 0
+        else:
+            a.lse_stride[:] = (heads * tokens, tokens)
+            a.starts = a.ends = 16  # the size does not depend on the call's pointers
+            ws_bytes = _lib.load().g4_kv8_attn_workspace_bytes(ctypes.byref(a))
+            a.workspace_bytes = ws_bytes
+        return self._keep(key, (batch, bytes(a), (batch, heads, tokens), ws_bytes, chunk))
 
-        def fill(a):
-            a.q_stride[:], a.o_stride[:], a.lse_stride[:] = qs, sizes[0], sizes[1]
-            a.num_q_heads, a.window, a.max_seqlen_k = heads, window, max_k
-            a.workspace_bytes = self._kv8_workspace(a)
-
-        a = self._kv8(("attn", heads, window, max_k, *qs), layer, batch, tokens, fill)
-        self._rows(a, batch, slots, starts, ends)
-        self._on_device()
-        out = torch.empty((batch, tokens, heads, d), dtype=torch.bfloat16, device=self.device)
-        lse = torch.empty((batch, heads, tokens), dtype=torch.float32, device=self.device)
-        ws = _workspace(a.workspace_bytes, self.device)
-        a.q, a.o, a.lse, a.workspace = q.data_ptr(), out.data_ptr(), lse.data_ptr(), ws.data_ptr()
-        self._launch(_lib.load().g4_kv8_attn, ctypes.byref(a))
-        return out, lse
-
-    def _kv8_workspace(self, a) -> int:
-        a.starts, a.ends = 16, 16  # the size does not depend on the call's pointers
-        n = _lib.load().g4_kv8_attn_workspace_bytes(ctypes.byref(a))
-        a.starts = a.ends = None
-        return n
-
-    def _chunk(self, layer, q, slots, starts, ends, window, max_k):
+    def _chunk(self, a, layer, q, out, slots):
         batch, tokens, heads, d = q.shape
+        if q.data_ptr() % 16:
+            raise ValueError("q must be 16-byte aligned")
+        window, max_k = a.window, a.max_seqlen_k
         keys = tokens + (min(max_k, window) if window else max_k) - 1  # most a row can see
         total = batch * tokens
-        # checked before the first launch, like the direct path's operands
-        if q.data_ptr() % 16 or any(s % 8 for s in _strides(q)):
-            raise ValueError("q must be 16-byte aligned with strides that are multiples of 8")
-
-        def fill(a):
-            a.num_q_heads, a.window, a.max_seqlen_k = heads, window, max_k
-            a.o_stride[:] = (heads * tokens * d, heads * d, d)
-            a.lse_stride[:] = (tokens, total)
-
-        a = self._kv8(("chunk", heads, window, max_k), layer, batch, tokens, fill)
-        self._rows(a, batch, slots, starts, ends)
-        self._on_device()
         lib = _lib.load()
         plan = torch.empty(4 * batch + 2, dtype=torch.int32, device=self.device)
         cu_q, cu_k = plan[:batch + 1], plan[batch + 1:2 * batch + 2]
         first, last = plan[2 * batch + 2:3 * batch + 2], plan[3 * batch + 2:]
         self._launch(lib.g4_kv8_chunk_plan, ctypes.byref(a), cu_q.data_ptr(), cu_k.data_ptr(),
                      first.data_ptr(), last.data_ptr())
-        shape = (batch * keys, self.num_kv_heads, d)
-        k = torch.empty(shape, dtype=torch.bfloat16, device=self.device)
-        v = torch.empty(shape, dtype=torch.bfloat16, device=self.device)
-        self._read(layer, slots, first, last, k, v, [8, self.num_kv_heads * d, d], batch, keys,
-                   cu_k)
-        out = torch.empty((batch, tokens, heads, d), dtype=torch.bfloat16, device=self.device)
+        k = torch.empty((batch * keys, self.num_kv_heads, d), dtype=torch.bfloat16,
+                        device=self.device)
+        v = torch.empty_like(k)
+        self._read(layer, slots, first, last, k, v, batch, keys, cu_k)
         with torch.cuda.device(self.device):
             _, lse = ops.attn_fwd(q.reshape(total, heads, d), k, v, window=window,
                                   cu_seqlens_q=cu_q, cu_seqlens_k=cu_k, max_seqlen_q=tokens,
                                   max_seqlen_k=keys, out=out.view(total, heads, d))
-        a.o, a.lse = out.data_ptr(), lse.data_ptr()
+        a.lse = lse.data_ptr()
         self._launch(lib.g4_kv8_pad_rows, ctypes.byref(a))
-        return out, lse.view(heads, batch, tokens).transpose(0, 1)
+        return lse.view(heads, batch, tokens).transpose(0, 1)
 
     # ----------------------------------------------------------------------------
     # pages
@@ -385,11 +389,9 @@ class PagedKVCache8:
         batch = self._page_rows(slots, "slots")
         if isinstance(counts, int):
             counts = torch.full((batch,), counts, dtype=torch.int32, device=self.device)
-        _ints(counts, batch, "counts", self.device)
-        span = torch.empty((2, batch), dtype=torch.int32, device=self.device)
-        starts, ends = span[0], span[1]
+        self._ints(counts, batch, "counts")
+        starts, ends = torch.empty((2, batch), dtype=torch.int32, device=self.device).unbind(0)
         if batch:
-            self._on_device()
             a, _ = self._pages(batch, slots)
             a.counts, a.starts, a.ends = counts.data_ptr(), starts.data_ptr(), ends.data_ptr()
             self._launch(_lib.load().g4_pages_extend, ctypes.byref(a))
@@ -399,9 +401,8 @@ class PagedKVCache8:
         """Make each child (an empty slot) a copy of its parent: whole pages are
         shared, a partly filled last page is copied in every layer."""
         batch = self._page_rows(parents, "parents")
-        _ints(children, batch, "children", self.device)
+        self._ints(children, batch, "children")
         if batch:
-            self._on_device()
             a, _ws = self._pages(batch, parents, children, workspace=True)
             self._launch(_lib.load().g4_pages_fork, ctypes.byref(a))
 
@@ -419,14 +420,12 @@ class PagedKVCache8:
     def _free(self, slots, window) -> None:
         batch = self._page_rows(slots, "slots")
         if batch:
-            self._on_device()
             a, _ = self._pages(batch, slots)
             a.window = window
             self._launch(_lib.load().g4_pages_free, ctypes.byref(a))
 
     def compact(self) -> None:
         """Move the live pages to the lowest ids, so that the pool's end is free."""
-        self._on_device()
         a, _ws = self._pages(0, workspace=True)
         self._launch(_lib.load().g4_pages_compact, ctypes.byref(a))
 
@@ -434,15 +433,14 @@ class PagedKVCache8:
         """Copy page ``src[i]`` to page ``dst[i]`` in every layer, with its scales;
         tables and refcounts stay.  A pair with a bad id, with a destination that an
         earlier pair has too, or whose destination is any pair's source is left out."""
-        batch = _ints(src, None, "src", self.device).shape[0]
-        _ints(dst, batch, "dst", self.device)
+        batch = self._ints(src, None, "src").shape[0]
+        self._ints(dst, batch, "dst")
         if batch:
-            self._on_device()
             a, _ = self._pages(batch, src, dst)
             self._launch(_lib.load().g4_pages_copy, ctypes.byref(a))
 
     def _page_rows(self, t: torch.Tensor, name: str) -> int:
-        batch = _ints(t, None, name, self.device).shape[0]
+        batch = self._ints(t, None, name).shape[0]
         if batch > MAX_ROWS:
             raise UnsupportedB200Path(f"at most {MAX_ROWS} rows per call")
         return batch

@@ -388,6 +388,7 @@ typedef struct g4_kv8_args {
   int32_t num_q_heads;
   int32_t window;       /* 0: every earlier key; W > 0: keys k > position - W */
   int32_t max_seqlen_k; /* upper bound of ends; a row beyond it is empty */
+  int32_t device;       /* CUDA device of the pointers and the stream; -1: the current one */
   void* workspace;
   size_t workspace_bytes;
 } g4_kv8_args;
@@ -459,6 +460,7 @@ typedef struct g4_pages_args {
   int32_t* ends;         /* extend, out: one past its last (= start: not served) */
   int32_t window;        /* free: 0 frees the rows; W > 0 only the leading pages that no
                             token from position `length` on sees through the window */
+  int32_t device;        /* CUDA device of the pointers and the stream; -1: the current one */
   void* workspace;
   size_t workspace_bytes;
 } g4_pages_args;
