@@ -20,8 +20,7 @@ namespace g4 {
 
 namespace {
 
-constexpr int kChunk = 16;         // elements per thread and step: 32 bytes of bf16
-constexpr int kAppendSteps = 8;    // chunks a thread holds in registers
+constexpr int kChunk = 8;          // elements per thread and step: 16 bytes of bf16, 8 of codes
 
 // Largest magnitude (bf16 bits, non-finite ignored) of two packed values, kept per half.
 __device__ __forceinline__ uint32_t max_finite2(uint32_t m, uint32_t x) {
@@ -42,6 +41,26 @@ __device__ __forceinline__ float pow2f(int e) {  // -126 <= e <= 127
   return __uint_as_float(static_cast<uint32_t>(e + 127) << 23);
 }
 
+// Codes of four finite values that the block's scale covers.
+template <bool kInt8>
+__device__ __forceinline__ uint32_t pack4_fast(float a, float b, float c, float d, float back) {
+  if constexpr (kInt8) {
+    // 1.5 * 2^23 + y rounds y to an integer (ties to even); its low byte is the code
+    const float magic = 12582912.f;
+    const uint32_t ab = __byte_perm(__float_as_uint(fmaf(a, back, magic)),
+                                    __float_as_uint(fmaf(b, back, magic)), 0x0040);
+    const uint32_t cd = __byte_perm(__float_as_uint(fmaf(c, back, magic)),
+                                    __float_as_uint(fmaf(d, back, magic)), 0x0040);
+    return __byte_perm(ab, cd, 0x5410);
+  } else {
+    uint16_t lo, hi;  // the first source is the upper byte
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(b * back), "f"(a * back));
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(d * back), "f"(c * back));
+    return static_cast<uint32_t>(lo) | (static_cast<uint32_t>(hi) << 16);
+  }
+}
+
+// The same for any values: infinities saturate, NaN becomes 0.
 template <bool kInt8>
 __device__ __forceinline__ uint32_t pack4(float a, float b, float c, float d) {
   if constexpr (kInt8) {
@@ -69,7 +88,8 @@ __device__ __forceinline__ uint32_t bf16_pair(float lo, float hi) {
 
 }  // namespace
 
-template <int D, bool kInt8>
+// kSteps: chunks a thread holds (1 for single tokens, else 8; 16 for the largest pages).
+template <int D, bool kInt8, int kSteps>
 __global__ void __launch_bounds__(512) kv8_append_kernel(const Kv8StoreParams p) {
   __shared__ uint32_t red[16];
   pdl_enter();
@@ -84,6 +104,22 @@ __global__ void __launch_bounds__(512) kv8_append_kernel(const Kv8StoreParams p)
   const int a = max(row.start, page_pos);
   const int n = min(row.start + row.n, page_pos + c.page) - a;  // new tokens of this page
   if (n <= 0) return;
+  constexpr int kPerRow = D / kChunk;
+  const int64_t* xs = is_v ? p.v_stride : p.k_stride;
+  const __nv_bfloat16* x = (is_v ? p.v : p.k) + static_cast<int64_t>(b) * xs[0] +
+                           static_cast<int64_t>(a - row.start) * xs[1] +
+                           static_cast<int64_t>(head) * xs[2];
+  // the values first: the page's lookup below runs while they are on their way
+  uint4 in[kSteps];
+#pragma unroll
+  for (int s = 0; s < kSteps; ++s) {
+    const int u = threadIdx.x + s * blockDim.x;
+    in[s] = make_uint4(0u, 0u, 0u, 0u);
+    if (u < n * kPerRow)
+      in[s] = *reinterpret_cast<const uint4*>(x + static_cast<int64_t>(u / kPerRow) * xs[1] +
+                                              (u % kPerRow) * kChunk);
+  }
+  const int page = kv8_page(c, row.slot, page_pos);
   // a slot listed twice: the first row writes it, later ones are left out (two
   // CTAs would race on the page's scale)
   if (p.rows.slots) {
@@ -94,45 +130,27 @@ __global__ void __launch_bounds__(512) kv8_append_kernel(const Kv8StoreParams p)
       return;
     }
   }
-  const int page = kv8_page(c, row.slot, page_pos);
   if (page < 0) {
     if (threadIdx.x == 0 && p.status) atomicOr(p.status, kKv8BadIndex);
     return;
   }
-  constexpr int kPerRow = D / kChunk;
-  const int64_t* xs = is_v ? p.v_stride : p.k_stride;
-  const __nv_bfloat16* x = (is_v ? p.v : p.k) + static_cast<int64_t>(b) * xs[0] +
-                           static_cast<int64_t>(a - row.start) * xs[1] +
-                           static_cast<int64_t>(head) * xs[2];
   const int64_t block = static_cast<int64_t>(page) * c.heads + head;
   uint8_t* codes = (is_v ? c.v : c.k) + block * c.page * D;
   float* scale = (is_v ? c.v_scale : c.k_scale) + block;
   const int held = a - page_pos;  // earlier tokens of the page
   const float old_scale = held > 0 ? *scale : 0.f;
-
-  uint4 in[kAppendSteps][2];
   uint32_t m = 0;
 #pragma unroll
-  for (int s = 0; s < kAppendSteps; ++s) {
-    const int u = threadIdx.x + s * blockDim.x;
-    if (u < n * kPerRow) {
-      const uint4* src = reinterpret_cast<const uint4*>(
-          x + static_cast<int64_t>(u / kPerRow) * xs[1] + (u % kPerRow) * kChunk);
-      in[s][0] = src[0];
-      in[s][1] = src[1];
-    } else {
-      in[s][0] = in[s][1] = make_uint4(0u, 0u, 0u, 0u);
-    }
+  for (int s = 0; s < kSteps; ++s) {
+    m = __vmaxu2(__vmaxu2(m, in[s].x & 0x7fff7fffu), in[s].y & 0x7fff7fffu);
+    m = __vmaxu2(__vmaxu2(m, in[s].z & 0x7fff7fffu), in[s].w & 0x7fff7fffu);
   }
+  const bool odd = (m >> 16) >= 0x7f80u || (m & 0xffffu) >= 0x7f80u;  // an infinity or NaN
+  if (odd) {
+    m = 0;
 #pragma unroll
-  for (int s = 0; s < kAppendSteps; ++s) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      m = max_finite2(m, in[s][h].x);
-      m = max_finite2(m, in[s][h].y);
-      m = max_finite2(m, in[s][h].z);
-      m = max_finite2(m, in[s][h].w);
-    }
+    for (int s = 0; s < kSteps; ++s)
+      m = max_finite2(max_finite2(max_finite2(max_finite2(m, in[s].x), in[s].y), in[s].z), in[s].w);
   }
   m = max(m >> 16, m & 0xffffu);
   m = __reduce_max_sync(0xffffffffu, m);
@@ -149,40 +167,40 @@ __global__ void __launch_bounds__(512) kv8_append_kernel(const Kv8StoreParams p)
     const float back = pow2f(-e);
     if (old_scale * back != 1.f) {
       for (int u = threadIdx.x; u < held * kPerRow; u += blockDim.x) {
-        uint4* at = reinterpret_cast<uint4*>(codes + static_cast<int64_t>(u) * kChunk);
-        const uint4 old = *at;
-        uint32_t w[4] = {old.x, old.y, old.z, old.w};
+        uint2* at = reinterpret_cast<uint2*>(codes + static_cast<int64_t>(u) * kChunk);
+        const uint2 old = *at;
+        uint32_t w[2] = {old.x, old.y};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < 2; ++i) {
           uint32_t lo, hi;
           kv8_to_half<kInt8>(w[i], lo, hi);
           const float2 l2 = half2_floats(lo), h2 = half2_floats(hi);
           w[i] = pack4<kInt8>(l2.x * old_scale * back, l2.y * old_scale * back,
                               h2.x * old_scale * back, h2.y * old_scale * back);
         }
-        *at = make_uint4(w[0], w[1], w[2], w[3]);
+        *at = make_uint2(w[0], w[1]);
       }
     }
   }
   const float back = pow2f(-e);
   codes += static_cast<int64_t>(held) * D;
 #pragma unroll
-  for (int s = 0; s < kAppendSteps; ++s) {
+  for (int s = 0; s < kSteps; ++s) {
     const int u = threadIdx.x + s * blockDim.x;
     if (u < n * kPerRow) {
-      uint32_t w[4];
+      const uint32_t r[4] = {in[s].x, in[s].y, in[s].z, in[s].w};
+      uint32_t w[2];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const uint32_t r[4] = {in[s][h].x, in[s][h].y, in[s][h].z, in[s][h].w};
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-          w[2 * h + i] = pack4<kInt8>(__uint_as_float(r[2 * i] << 16) * back,
-                                      __uint_as_float(r[2 * i] & 0xffff0000u) * back,
-                                      __uint_as_float(r[2 * i + 1] << 16) * back,
-                                      __uint_as_float(r[2 * i + 1] & 0xffff0000u) * back);
+      for (int i = 0; i < 2; ++i)
+      {
+        const float v[4] = {__uint_as_float(r[2 * i] << 16),
+                            __uint_as_float(r[2 * i] & 0xffff0000u),
+                            __uint_as_float(r[2 * i + 1] << 16),
+                            __uint_as_float(r[2 * i + 1] & 0xffff0000u)};
+        w[i] = odd ? pack4<kInt8>(v[0] * back, v[1] * back, v[2] * back, v[3] * back)
+                   : pack4_fast<kInt8>(v[0], v[1], v[2], v[3], back);
       }
-      *reinterpret_cast<uint4*>(codes + static_cast<int64_t>(u) * kChunk) =
-          make_uint4(w[0], w[1], w[2], w[3]);
+      *reinterpret_cast<uint2*>(codes + static_cast<int64_t>(u) * kChunk) = make_uint2(w[0], w[1]);
     }
   }
   if (threadIdx.x == 0) *scale = pow2f(e);
@@ -193,67 +211,69 @@ __global__ void __launch_bounds__(512) kv8_append_kernel(const Kv8StoreParams p)
 // nothing.  Bound: HBM, 1 byte read and 2 written per element.
 // Packed output: so are the rows behind the last segment that a 128-key tile of the
 // forward may load (masked there, but 0 * NaN would not be 0).
-constexpr int kReadTokens = 16;  // tokens per CTA
+constexpr int kReadTokens = 16;  // tokens per CTA, K and V
 constexpr int kReadTail = 128;
 template <int D, bool kInt8>
 __global__ void __launch_bounds__(128) kv8_read_kernel(const Kv8StoreParams p) {
   pdl_enter();
-  const int b = blockIdx.z >> 1;
-  const bool is_v = blockIdx.z & 1;
+  const int b = blockIdx.z;
   const int head = blockIdx.y;
   const Kv8Cache& c = p.cache;
   const Kv8Row row = kv8_row(c, p.rows, b, INT32_MAX);
   const int base = p.out_rows ? p.out_rows[b] : 0;
   int len = p.out_rows ? p.out_rows[b + 1] - base : p.rows.tokens;
   if (p.out_rows && b == p.rows.batch - 1) len += min(kReadTail, p.out_total - base - len);
-  __nv_bfloat16* out = (is_v ? p.v_out : p.k_out) +
-                       (p.out_rows ? static_cast<int64_t>(base) * p.out_stride[1]
-                                   : static_cast<int64_t>(b) * p.out_stride[0]) +
-                       static_cast<int64_t>(head) * p.out_stride[2];
-  const uint8_t* pool = is_v ? c.v : c.k;
-  const float* scales = is_v ? c.v_scale : c.k_scale;
+  const int64_t out_at = (p.out_rows ? static_cast<int64_t>(base) * p.out_stride[1]
+                                     : static_cast<int64_t>(b) * p.out_stride[0]) +
+                         static_cast<int64_t>(head) * p.out_stride[2];
   constexpr int kPerRow = D / kChunk;
   constexpr int kRows = 128 / kPerRow;  // tokens per step
   constexpr int kSteps = kReadTokens / kRows;
   const int t0 = blockIdx.x * kReadTokens;
   if (t0 >= len) return;
-  uint4 w[kSteps];
-  float s[kSteps];
+  const int at = threadIdx.x / kPerRow, chunk = (threadIdx.x % kPerRow) * kChunk;
+  int page[kSteps];
 #pragma unroll
   for (int i = 0; i < kSteps; ++i) {
-    const int t = t0 + i * kRows + threadIdx.x / kPerRow;
-    w[i] = make_uint4(0u, 0u, 0u, 0u);
-    s[i] = 0.f;
-    if (t < min(len, row.n)) {
-      const int pos = row.start + t;
-      const int page = kv8_page(c, row.slot, pos);
-      if (page >= 0) {
-        const int64_t block = static_cast<int64_t>(page) * c.heads + head;
-        s[i] = scales[block];
-        w[i] = *reinterpret_cast<const uint4*>(
-            pool + (block * c.page + (pos & (c.page - 1))) * D + (threadIdx.x % kPerRow) * kChunk);
-      }
+    const int t = t0 + i * kRows + at;
+    page[i] = t < min(len, row.n) ? kv8_page(c, row.slot, row.start + t) : -1;
+  }
+  uint2 w[2][kSteps];
+  float s[2][kSteps];
+#pragma unroll
+  for (int i = 0; i < kSteps; ++i) {
+    const int pos = row.start + t0 + i * kRows + at;
+    const int64_t block = static_cast<int64_t>(max(page[i], 0)) * c.heads + head;
+    const int64_t from = (block * c.page + (pos & (c.page - 1))) * D + chunk;
+    w[0][i] = w[1][i] = make_uint2(0u, 0u);
+    s[0][i] = s[1][i] = 0.f;  // a hole reads as exact zeros: its codes and scales are zero here
+    if (page[i] >= 0) {
+      w[0][i] = __ldcs(reinterpret_cast<const uint2*>(c.k + from));
+      w[1][i] = __ldcs(reinterpret_cast<const uint2*>(c.v + from));
+      s[0][i] = c.k_scale[block];
+      s[1][i] = c.v_scale[block];
     }
   }
 #pragma unroll
   for (int i = 0; i < kSteps; ++i) {
-    const int t = t0 + i * kRows + threadIdx.x / kPerRow;
+    const int t = t0 + i * kRows + at;
     if (t >= len) break;
-    const uint32_t r[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
-    uint32_t o[8];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      uint32_t lo, hi;
-      kv8_to_half<kInt8>(r[j], lo, hi);
-      const float2 l2 = half2_floats(lo), h2 = half2_floats(hi);
-      o[2 * j] = bf16_pair(l2.x * s[i], l2.y * s[i]);
-      o[2 * j + 1] = bf16_pair(h2.x * s[i], h2.y * s[i]);
+    for (int kv = 0; kv < 2; ++kv) {
+      const uint32_t r[2] = {w[kv][i].x, w[kv][i].y};
+      uint32_t o[4];
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        uint32_t lo, hi;
+        kv8_to_half<kInt8>(r[j], lo, hi);
+        const float2 l2 = half2_floats(lo), h2 = half2_floats(hi);
+        o[2 * j] = bf16_pair(l2.x * s[kv][i], l2.y * s[kv][i]);
+        o[2 * j + 1] = bf16_pair(h2.x * s[kv][i], h2.y * s[kv][i]);
+      }
+      *reinterpret_cast<uint4*>((kv ? p.v_out : p.k_out) + out_at +
+                                static_cast<int64_t>(t) * p.out_stride[1] + chunk) =
+          make_uint4(o[0], o[1], o[2], o[3]);
     }
-    // a hole (no page) reads as exact zeros: its codes and scale are zero here
-    uint4* dst = reinterpret_cast<uint4*>(out + static_cast<int64_t>(t) * p.out_stride[1] +
-                                          (threadIdx.x % kPerRow) * kChunk);
-    dst[0] = make_uint4(o[0], o[1], o[2], o[3]);
-    dst[1] = make_uint4(o[4], o[5], o[6], o[7]);
   }
 }
 
@@ -315,20 +335,24 @@ template <int D, bool kInt8>
 int append(const Kv8StoreParams& p, cudaStream_t stream) {
   const int page = p.cache.page, tokens = p.rows.tokens;
   const int pages = tokens > 1 ? (tokens - 2) / page + 2 : 1;  // most that `tokens` can touch
-  // four chunks per thread where the page is large enough, eight at the largest
   const int chunks = (tokens < page ? tokens : page) * (D / kChunk);
-  int threads = (chunks / 4 + 31) / 32 * 32;
-  threads = threads < 32 ? 32 : threads > 512 ? 512 : threads;
-  return static_cast<int>(launch_chained(kv8_append_kernel<D, kInt8>,
-                                         dim3(pages, p.cache.heads, 2 * p.rows.batch),
-                                         dim3(threads), 0, stream, p));
+  const dim3 grid(pages, p.cache.heads, 2 * p.rows.batch);
+  const auto threads = [&](int steps) { return dim3((chunks / steps + 31) / 32 * 32); };
+  cudaError_t e;
+  if (chunks <= 512)
+    e = launch_chained(kv8_append_kernel<D, kInt8, 1>, grid, threads(1), 0, stream, p);
+  else if (chunks <= 4096)
+    e = launch_chained(kv8_append_kernel<D, kInt8, 8>, grid, threads(8), 0, stream, p);
+  else
+    e = launch_chained(kv8_append_kernel<D, kInt8, 16>, grid, threads(16), 0, stream, p);
+  return static_cast<int>(e);
 }
 template <int D, bool kInt8>
 int read(const Kv8StoreParams& p, cudaStream_t stream) {
   const int most = p.rows.tokens + (p.out_rows ? kReadTail : 0);
   return static_cast<int>(launch_chained(
       kv8_read_kernel<D, kInt8>,
-      dim3((most + kReadTokens - 1) / kReadTokens, p.cache.heads, 2 * p.rows.batch),
+      dim3((most + kReadTokens - 1) / kReadTokens, p.cache.heads, p.rows.batch),
       dim3(128), 0, stream, p));
 }
 }  // namespace
