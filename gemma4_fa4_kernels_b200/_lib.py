@@ -218,6 +218,7 @@ class G4Kv8Args(ctypes.Structure):
 G4_PAGES_EXHAUSTED = 1
 G4_PAGES_ROW_FULL = 2
 G4_PAGES_BAD_INDEX = 4
+G4_KV8_DEVICE_WAIT = 8
 
 
 class G4PagesArgs(ctypes.Structure):

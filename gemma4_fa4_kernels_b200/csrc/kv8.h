@@ -24,16 +24,19 @@
 namespace g4 {
 
 constexpr int kKv8MaxBatch = 1024;  // rows of one call (their plan sits in shared memory)
+constexpr int kKv8MaxSmem = 232448; // dynamic shared memory per CTA
 constexpr int kKv8Tile = 32;        // keys per attention tile: two pieces of 16, each in one page
 // exponents of a block's scale 2^e: 2^e and 2^-e are both normal fp32 values, and
 // the largest finite bf16 value fits 448 * 2^120 and 127 * 2^122
 constexpr int kKv8MinExp = -100;
 constexpr int kKv8MaxExp = 122;
 
+
 enum Kv8Status : int {
   kKv8PoolExhausted = 1,    // no free page left for a row
   kKv8RowFull = 2,          // a row's table is full
   kKv8BadIndex = 4,         // slot, page or count out of range, or the same one twice
+  kKv8DeviceWait = 8,       // a bounded wait expired: the call's results are invalid
 };
 
 struct Kv8Cache {
@@ -116,6 +119,7 @@ struct Kv8AttnParams {
   int max_k;                // rows that end past it count as empty
   int group;                // query heads per KV head
   int cols;                 // (token, query head) columns of one item (Kv8AttnShape)
+  int tile;                 // keys per tile of the list
   int col_groups;           // ceil(tokens * group / cols)
   const __nv_bfloat16* q;   // (batch, token, head) strides in elements
   int64_t q_stride[3];
@@ -126,16 +130,20 @@ struct Kv8AttnParams {
   // partial results (workspace): two per run, [run][head, tail]
   float* part_o;            // [slot][cols][head_dim]
   float4* part_ml;          // [slot][cols]: (shift of O, max, sum, -)
+  int* status;              // nullable
   int* plan;                // {runs, tiles, -, -}, the rows' plans (int4 each), their first tiles
 };
 // The kernel's launch shape for a row's number of (token, query head) columns.
 struct Kv8AttnShape {
   int cols;                 // columns one pass over the codes serves
+  int tile;                 // keys per tile
   int runs;                 // runs per CTA
   int out_floats;           // floats of a partial O
 };
 Kv8AttnShape kv8_attn_shape(int d, int64_t columns);
+Kv8AttnShape kv8_wide_shape(int d, int64_t columns);  // kv8_wide.cu
 int launch_kv8_attn(int d, bool int8, const Kv8AttnParams& p, int ctas, cudaStream_t stream);
+int launch_kv8_wide(int d, bool int8, const Kv8AttnParams& p, int ctas, cudaStream_t stream);
 int launch_kv8_merge(int d, const Kv8AttnParams& p, int ctas, cudaStream_t stream);
 
 // ---- append, read back, chunks of prompts (kv8_store.cu) ----

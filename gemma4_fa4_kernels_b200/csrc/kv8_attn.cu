@@ -1,5 +1,6 @@
-// Attention over the 8-bit paged KV cache for sm_100a: one to a few query tokens
-// per sequence (decode, drafted tokens), any batch of ragged lengths.
+// Attention over the 8-bit paged KV cache for sm_100a: up to 8 (query token, query
+// head) columns per KV head and sequence (decode), any batch of ragged lengths.  More
+// columns: kv8_wide.cu.
 //
 //   S = Q K^T,  P = softmax(S masked),  O = P V,  K = s_k * k8,  V = s_v * v8
 // with s_k, s_v one scale per (page, KV head).  The scales stay outside the
@@ -45,24 +46,19 @@
 #include <algorithm>
 
 #include "g4_kernels.h"
-#include "g4_sm100.cuh"
-#include "kv8.h"
+#include "kv8_list.cuh"
 
 namespace g4 {
 
 namespace {
 
-constexpr float kShiftUp = 11.f;    // log2 of the factor on P
-constexpr float kStale = 3.f;       // log2 by which O's maximum may lag before a rescale
-
-// One launch shape: kTeam warps share a run, kBlocks blocks of 8 columns are
-// served by one pass over the codes.
-template <int kD, int kTeam_, int kBlocks_, int kWarps_, int kBufs_>
+// A launch shape: kTeam warps share a run; one pass over the codes serves 8 columns.
+template <int kD, int kTeam_, int kWarps_, int kBufs_>
 struct AttnShape {
-  static constexpr int D = kD, kTeam = kTeam_, kBlocks = kBlocks_, kWarps = kWarps_;
+  static constexpr int D = kD, kTeam = kTeam_, kWarps = kWarps_;
   static constexpr int kTeams = kWarps / kTeam;        // runs per CTA
   static constexpr int kThreads = kWarps * 32;
-  static constexpr int kCols = 8 * kBlocks;
+  static constexpr int kCols = 8;
   static constexpr int kDims = D / kTeam;              // dims per warp
   static constexpr int kRow = kDims + 16;              // bytes per key row in a buffer
   static constexpr int kBuf = 16 * kRow;
@@ -75,7 +71,7 @@ struct AttnShape {
   static constexpr int kOutRow = D + 4;                // and of its columns in shared memory
   static constexpr int kRingBytes = kWarps * kRing;
   static constexpr int kSwaps = kTeam > 1 ? 2 : 1;     // copies of the S buffers
-  static constexpr int kExchange = kWarps * kSwaps * kBlocks * 1024;
+  static constexpr int kExchange = kWarps * kSwaps * 1024;
   static constexpr int kStats = kTeams * kCols * 16;
   static constexpr int kTails = kTeams * 4 * 4;
   static_assert(kRingBytes >= kTeams * kCols * kOutRow * 4, "the runs' ends are summed in the ring's place");
@@ -84,46 +80,6 @@ struct AttnShape {
            4 * kWarps;
   }
 };
-
-// A tile's place: row, item within the row, tile.
-struct Place {
-  int b;
-  int item;     // active items (queries present) first, then the padded column groups
-  int tile;     // absolute tile index (32 keys)
-  int left;     // tiles left in the item
-};
-
-struct RowPlan {  // shared memory, one per row
-  int slot;
-  int start;
-  int n;
-  int lo;       // first visible key of the row
-};
-
-template <int kCols>
-__device__ __forceinline__ int active_groups(const RowPlan& r, int group) {
-  return (r.n * group + kCols - 1) / kCols;
-}
-__device__ __forceinline__ int row_tiles(const RowPlan& r) {
-  return r.n > 0 ? (r.start + r.n + kKv8Tile - 1) / kKv8Tile - r.lo / kKv8Tile : 1;
-}
-__device__ __forceinline__ RowPlan row_plan(const Kv8AttnParams& p, int b) {
-  const Kv8Row r = kv8_row(p.cache, p.rows, b, p.max_k);
-  RowPlan rp;
-  rp.slot = r.slot;
-  rp.start = r.start;
-  rp.n = r.n;
-  rp.lo = p.window > 0 ? max(0, r.start - p.window + 1) : 0;
-  return rp;
-}
-
-// Run i of n over `total` tiles begins at floor(i * total / n); n <= total.
-__device__ __forceinline__ int run_begin(int i, int n, int total) {
-  return static_cast<int>(static_cast<int64_t>(i) * total / n);
-}
-__device__ __forceinline__ int run_of(int tile, int n, int total) {
-  return static_cast<int>((static_cast<int64_t>(tile + 1) * n - 1) / total);
-}
 
 __device__ __forceinline__ void mma_16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
                                           uint32_t b1) {
@@ -147,77 +103,14 @@ __device__ __forceinline__ void cp4_z(uint32_t dst, const void* src, int bytes) 
                : "memory");
 }
 
-// Exponent of the power of two that brings a column's Q to [2^13, 2^14); zeros and
-// non-finite values stay.
-__device__ __forceinline__ int q_exponent(float amax) {
-  const int bits = static_cast<int>(__float_as_uint(amax) >> 23);
-  if (bits == 0 || bits == 255) return 0;
-  return min(13 - (bits - 127), 100);
-}
-
 // 16-byte chunk of a V row (of the warp's dims) that thread row g takes in step i.
 __device__ __forceinline__ int v_chunk(int g, int i) { return (g & 1) * 4 + (g >> 1) + 8 * i; }
-
-// Factor from a held O (sum * 2^(kShiftUp - m_shift)) to the output; 0 without a key.
-__device__ __forceinline__ float out_factor(float m_shift, float m, float l) {
-  return l == 0.f || m_shift == -INFINITY ? 0.f : ex2(m_shift - kShiftUp - m) / l;
-}
-
-// Where column `col` of KV head `h` in row b goes: 16 consecutive dims, and its LSE.
-__device__ __forceinline__ void put_out(const Kv8AttnParams& p, int b, int h, int col, int dim,
-                                        const float (&v)[16], float f) {
-  const int tok = col / p.group;
-  if (tok >= p.rows.tokens) return;
-  uint32_t w[8];
-#pragma unroll
-  for (int x = 0; x < 8; ++x) w[x] = pack_bf16x2(v[2 * x] * f, v[2 * x + 1] * f);
-  uint4* dst = reinterpret_cast<uint4*>(
-      p.o + static_cast<int64_t>(b) * p.o_stride[0] + static_cast<int64_t>(tok) * p.o_stride[1] +
-      static_cast<int64_t>(h * p.group + col - tok * p.group) * p.o_stride[2] + dim);
-  dst[0] = make_uint4(w[0], w[1], w[2], w[3]);
-  dst[1] = make_uint4(w[4], w[5], w[6], w[7]);
-}
-// The same for four dims.
-__device__ __forceinline__ void put_dims(const Kv8AttnParams& p, int b, int h, int col, int dim,
-                                         const float4& v, float f) {
-  const int tok = col / p.group;
-  *reinterpret_cast<uint2*>(
-      p.o + static_cast<int64_t>(b) * p.o_stride[0] + static_cast<int64_t>(tok) * p.o_stride[1] +
-      static_cast<int64_t>(h * p.group + col - tok * p.group) * p.o_stride[2] + dim) =
-      make_uint2(pack_bf16x2(v.x * f, v.y * f), pack_bf16x2(v.z * f, v.w * f));
-}
-__device__ __forceinline__ void put_lse(const Kv8AttnParams& p, int b, int h, int col, float m,
-                                        float l) {
-  const int tok = col / p.group;
-  if (tok >= p.rows.tokens) return;
-  p.lse[static_cast<int64_t>(b) * p.lse_stride[0] +
-        static_cast<int64_t>(h * p.group + col - tok * p.group) * p.lse_stride[1] + tok] =
-      l > 0.f ? (m + __log2f(l)) * kLn2 : (l == 0.f ? -INFINITY : l);
-}
-
-// Running (shift of O, max, sum) <- with another part's; returns the factors on both Os.
-__device__ __forceinline__ float2 join(float& m_shift, float& m, float& l, const float4 st) {
-  const float ms = fmaxf(m_shift, st.x), mn = fmaxf(m, st.y);
-  const float fa = m_shift == -INFINITY ? 0.f : ex2(m_shift - ms);
-  const float fb = st.x == -INFINITY ? 0.f : ex2(st.x - ms);
-  l = (m == -INFINITY ? l : l * ex2(m - mn)) + (st.y == -INFINITY ? st.z : st.z * ex2(st.y - mn));
-  m_shift = ms;
-  m = mn;
-  return make_float2(fa, fb);
-}
-
-__device__ __forceinline__ void axpby(float4& v, const float2 f, const float4& o) {
-  v.x = v.x * f.x + o.x * f.y;
-  v.y = v.y * f.x + o.y * f.y;
-  v.z = v.z * f.x + o.z * f.y;
-  v.w = v.w * f.x + o.w * f.y;
-}
 
 }  // namespace
 
 template <typename Cfg, bool kInt8>
 __global__ void __launch_bounds__(Cfg::kThreads, 1) kv8_attn_kernel(const Kv8AttnParams p) {
-  constexpr int D = Cfg::D, kTeam = Cfg::kTeam, kBlocks = Cfg::kBlocks, kCols = Cfg::kCols;
+  constexpr int D = Cfg::D, kTeam = Cfg::kTeam, kCols = Cfg::kCols;
   extern __shared__ __align__(16) uint8_t smem[];
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int g = lane >> 2, t = lane & 3;
@@ -232,109 +125,20 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1) kv8_attn_kernel(const Kv8Att
   int* scan = prefix + p.rows.batch + 1;
 
   pdl_enter();
-  // ---- plan: checked rows, their tiles, the prefix sum over rows ----
   const int B = p.rows.batch, heads = p.cache.heads;
-  {
-    const int per = (B + Cfg::kThreads - 1) / Cfg::kThreads;  // rows per thread, consecutive
-    int mine = 0;
-    for (int j = 0; j < per; ++j) {
-      const int b = tid * per + j;
-      if (b >= B) break;
-      const RowPlan rp = row_plan(p, b);
-      rows[b] = rp;
-      const int act = active_groups<kCols>(rp, p.group);
-      mine += heads * (act * row_tiles(rp) + p.col_groups - act);
-    }
-    int inc = mine;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int up = __shfl_up_sync(0xffffffffu, inc, o);
-      if (lane >= o) inc += up;
-    }
-    if (lane == 31) scan[warp] = inc;
-    __syncthreads();
-    int at = inc - mine;
-    for (int w = 0; w < warp; ++w) at += scan[w];
-    for (int j = 0; j < per; ++j) {
-      const int b = tid * per + j;
-      if (b >= B) break;
-      prefix[b] = at;
-      const RowPlan rp = rows[b];
-      const int act = active_groups<kCols>(rp, p.group);
-      at += heads * (act * row_tiles(rp) + p.col_groups - act);
-      if (b == B - 1) prefix[B] = at;
-    }
-    __syncthreads();
-  }
+  const auto row_at = [&](int b) { return rows[b]; };
+  const TileList<kKv8Tile, kCols, decltype(row_at)> list{p, row_at, prefix};
+  plan_rows<Cfg::kThreads>(p, list, prefix, scan, [&](int b, const RowPlan& r) { rows[b] = r; });
   const int total = prefix[B];
   const int runs = min(total, static_cast<int>(gridDim.x) * Cfg::kTeams);
-  if (blockIdx.x == 0) {  // for the merge
-    if (tid == 0) *reinterpret_cast<int4*>(p.plan) = make_int4(runs, total, 0, 0);
-    for (int b = tid; b < B; b += blockDim.x) {
-      reinterpret_cast<int4*>(p.plan)[1 + b] = reinterpret_cast<const int4*>(rows)[b];
-      p.plan[4 + 4 * B + b] = prefix[b];
-    }
-  }
+  if (blockIdx.x == 0 && tid == 0)
+    *reinterpret_cast<int4*>(p.plan) = make_int4(runs, total, 0, 0);
   const int W = blockIdx.x * Cfg::kTeams + team;
   const int w_begin = W < runs ? run_begin(W, runs, total) : 0;
   int todo = W < runs ? run_begin(W + 1, runs, total) - w_begin : 0;
 
-  // place of a list index
-  auto locate = [&](int x) {
-    int lo = 0, hi = B;  // prefix[lo] <= x < prefix[hi]
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (prefix[mid] <= x) lo = mid; else hi = mid;
-    }
-    Place pl;
-    pl.b = lo;
-    const RowPlan r = rows[lo];
-    const int nt = row_tiles(r);
-    const int act = heads * active_groups<kCols>(r, p.group);
-    const int rel = x - prefix[lo];
-    if (rel < act * nt) {
-      pl.item = rel / nt;
-      const int at = rel - pl.item * nt;
-      pl.tile = r.lo / kKv8Tile + at;
-      pl.left = nt - at;
-    } else {
-      pl.item = act + rel - act * nt;
-      pl.tile = 0;
-      pl.left = 1;
-    }
-    return pl;
-  };
-  auto next_item = [&](Place& pl) {
-    ++pl.item;
-    if (pl.item >= heads * p.col_groups) {
-      ++pl.b;
-      pl.item = 0;
-      if (pl.b >= B) {
-        pl.left = 0;
-        return;
-      }
-    }
-    const RowPlan r = rows[pl.b];
-    const bool act = pl.item < heads * active_groups<kCols>(r, p.group);
-    pl.tile = act ? r.lo / kKv8Tile : 0;
-    pl.left = act ? row_tiles(r) : 1;
-  };
-  // KV head and column group of an item
-  auto item_head = [&](int b, int item, int& head, int& cg) {
-    const int a = active_groups<kCols>(rows[b], p.group);
-    if (item < heads * a) {
-      head = item / a;
-      cg = item - head * a;
-    } else {
-      const int rest = p.col_groups - a;
-      const int j = item - heads * a;
-      head = j / rest;
-      cg = a + j - head * rest;
-    }
-  };
-
   // ---- the loading side: 16-key pieces in order K0a K0b V0a V0b K1a ... ----
-  Place ld = locate(w_begin);
+  Place ld = list.locate(w_begin);
   int ld_todo = todo;        // tiles not yet requested
   uint32_t ld_buf = 0;       // ring offset of the next request
   int ld_phase = 0;          // 0, 1: K halves; 2, 3: V halves
@@ -346,9 +150,9 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1) kv8_attn_kernel(const Kv8Att
   };
   auto set_item = [&]() {
     int cg;
-    item_head(ld.b, ld.item, ld_head, cg);
+    list.item_head(ld.b, ld.item, ld_head, cg);
     const RowPlan r = rows[ld.b];
-    const bool act = ld.item < heads * active_groups<kCols>(r, p.group);
+    const bool act = ld.item < list.active_items(r);
     ld_slot = r.slot;
     ld_lo = r.lo;
     ld_hi = act ? r.start + r.n : 0;
@@ -404,7 +208,7 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1) kv8_attn_kernel(const Kv8Att
         --ld_todo;
         ++ld.tile;
         if (--ld.left == 0) {
-          next_item(ld);
+          list.next_item(ld);
           if (ld_todo > 0) set_item();
         } else {
           ld_page[0] = ld_next[0];
@@ -420,148 +224,133 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1) kv8_attn_kernel(const Kv8Att
   for (int i = 0; i < Cfg::kBufs; ++i) request();
 
   // ---- the computing side ----
-  uint32_t qf[kBlocks][Cfg::kChunks][8];
-  float acc[kBlocks][Cfg::kTilesM][4];
-  float m_o[kBlocks][2], m_s[kBlocks][2], l_s[kBlocks][2];  // per column 2t, 2t + 1 of a block:
-                                                            // shift of O; max and sum of P
-  float q_back[kBlocks][2];               // log2(e) * 2^-e of the column's Q
-  int last_key[kBlocks][2];               // last visible key, -1: a padded column
-  Place pl = locate(w_begin);
+  uint32_t qf[Cfg::kChunks][8];
+  float acc[Cfg::kTilesM][4];
+  float m_o[2], m_s[2], l_s[2];           // columns 2t, 2t + 1: shift of O; max and sum of P
+  float q_back[2];               // log2(e) * 2^-e of the column's Q
+  int last_key[2];               // last visible key, -1: a padded column
+  Place pl = list.locate(w_begin);
   uint32_t use = 0;                       // ring offset of the next piece
   int head = 0, cg = 0, swap = 0;
 
   auto begin_item = [&]() {
-    item_head(pl.b, pl.item, head, cg);
+    list.item_head(pl.b, pl.item, head, cg);
     const RowPlan r = rows[pl.b];
+    // this thread's Q fragments: column g, dims of chunk c(t, i)
+    const int col = cg * kCols + g;
+    const int tok = col / p.group;
+    const bool have = tok < r.n;
+    const __nv_bfloat16* qp =
+        p.q + static_cast<int64_t>(pl.b) * p.q_stride[0] +
+        static_cast<int64_t>(have ? tok : 0) * p.q_stride[1] +
+        static_cast<int64_t>(head * p.group + (have ? col - tok * p.group : 0)) * p.q_stride[2];
+    // its raw values, and the column's largest magnitude over all D dims (the other
+    // warps' dims too, so that every warp of the team finds the same one)
+    uint4 raw[Cfg::kChunks][2];
+    uint32_t top = 0;
 #pragma unroll
-    for (int bl = 0; bl < kBlocks; ++bl) {
-      // this thread's Q fragments: column g, dims of chunk c(t, i)
-      const int col = cg * kCols + bl * 8 + g;
-      const int tok = col / p.group;
-      const bool have = tok < r.n;
-      const __nv_bfloat16* qp =
-          p.q + static_cast<int64_t>(pl.b) * p.q_stride[0] +
-          static_cast<int64_t>(have ? tok : 0) * p.q_stride[1] +
-          static_cast<int64_t>(head * p.group + (have ? col - tok * p.group : 0)) * p.q_stride[2];
-      // its raw values, and the column's largest magnitude over all D dims (the other
-      // warps' dims too, so that every warp of the team finds the same one)
-      uint4 raw[Cfg::kChunks][2];
-      uint32_t top = 0;
-#pragma unroll
-      for (int w = 0; w < kTeam; ++w) {
-#pragma unroll
-        for (int i = 0; i < Cfg::kChunks; ++i) {
-          const uint4* s = reinterpret_cast<const uint4*>(
-              qp + (part ^ (kTeam - 1 - w)) * Cfg::kDims + (2 * t + (i & 1) + 8 * (i >> 1)) * 16);
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            raw[i][h] = have ? s[h] : make_uint4(0u, 0u, 0u, 0u);
-            const uint4 x = raw[i][h];
-            top = __vmaxu2(__vmaxu2(top, x.x & 0x7fff7fffu), x.y & 0x7fff7fffu);
-            top = __vmaxu2(__vmaxu2(top, x.z & 0x7fff7fffu), x.w & 0x7fff7fffu);
-          }
-        }
-      }
-      top = max(top >> 16, top & 0xffffu);
-      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      const int e = q_exponent(__uint_as_float(top << 16));
-      // two factors: 2^e alone may leave the fp32 range for the smallest inputs
-      const float f1 = __uint_as_float(static_cast<uint32_t>(127 + e / 2) << 23);
-      const float f2 = __uint_as_float(static_cast<uint32_t>(127 + e - e / 2) << 23);
+    for (int w = 0; w < kTeam; ++w) {
 #pragma unroll
       for (int i = 0; i < Cfg::kChunks; ++i) {
+        const uint4* s = reinterpret_cast<const uint4*>(
+            qp + (part ^ (kTeam - 1 - w)) * Cfg::kDims + (2 * t + (i & 1) + 8 * (i >> 1)) * 16);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const uint32_t w[4] = {raw[i][h].x, raw[i][h].y, raw[i][h].z, raw[i][h].w};
-#pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            const float lo = __uint_as_float(w[x] << 16) * f1 * f2;
-            const float hi = __uint_as_float(w[x] & 0xffff0000u) * f1 * f2;
-            const __half2 v = __floats2half2_rn(lo, hi);
-            qf[bl][i][4 * h + x] = *reinterpret_cast<const uint32_t*>(&v);
-          }
+          raw[i][h] = have ? s[h] : make_uint4(0u, 0u, 0u, 0u);
+          const uint4 x = raw[i][h];
+          top = __vmaxu2(__vmaxu2(top, x.x & 0x7fff7fffu), x.y & 0x7fff7fffu);
+          top = __vmaxu2(__vmaxu2(top, x.z & 0x7fff7fffu), x.w & 0x7fff7fffu);
         }
       }
-#pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const int ce = __shfl_sync(0xffffffffu, e, (2 * t + x) * 4);  // column 2t + x
-        q_back[bl][x] = kLog2e * __uint_as_float(static_cast<uint32_t>(127 - ce) << 23);
-        const int ct = (cg * kCols + bl * 8 + 2 * t + x) / p.group;
-        last_key[bl][x] = ct < r.n ? r.start + ct : -1;
-        m_o[bl][x] = m_s[bl][x] = -INFINITY;
-        l_s[bl][x] = 0.f;
-      }
-#pragma unroll
-      for (int i = 0; i < Cfg::kTilesM; ++i)
-#pragma unroll
-        for (int x = 0; x < 4; ++x) acc[bl][i][x] = 0.f;
     }
+    top = max(top >> 16, top & 0xffffu);
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    const int e = q_exponent(__uint_as_float(top << 16));
+    // two factors: 2^e alone may leave the fp32 range for the smallest inputs
+    const float f1 = __uint_as_float(static_cast<uint32_t>(127 + e / 2) << 23);
+    const float f2 = __uint_as_float(static_cast<uint32_t>(127 + e - e / 2) << 23);
+#pragma unroll
+    for (int i = 0; i < Cfg::kChunks; ++i) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint32_t w[4] = {raw[i][h].x, raw[i][h].y, raw[i][h].z, raw[i][h].w};
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+          const float lo = __uint_as_float(w[x] << 16) * f1 * f2;
+          const float hi = __uint_as_float(w[x] & 0xffff0000u) * f1 * f2;
+          const __half2 v = __floats2half2_rn(lo, hi);
+          qf[i][4 * h + x] = *reinterpret_cast<const uint32_t*>(&v);
+        }
+      }
+    }
+#pragma unroll
+    for (int x = 0; x < 2; ++x) {
+      const int ce = __shfl_sync(0xffffffffu, e, (2 * t + x) * 4);  // column 2t + x
+      q_back[x] = kLog2e * __uint_as_float(static_cast<uint32_t>(127 - ce) << 23);
+      const int ct = (cg * kCols + 2 * t + x) / p.group;
+      last_key[x] = ct < r.n ? r.start + ct : -1;
+      m_o[x] = m_s[x] = -INFINITY;
+      l_s[x] = 0.f;
+    }
+#pragma unroll
+    for (int i = 0; i < Cfg::kTilesM; ++i)
+#pragma unroll
+      for (int x = 0; x < 4; ++x) acc[i][x] = 0.f;
   };
   auto column_sums = [&]() {  // over the warp's key rows
 #pragma unroll
-    for (int bl = 0; bl < kBlocks; ++bl)
+    for (int x = 0; x < 2; ++x)
 #pragma unroll
-      for (int x = 0; x < 2; ++x)
-#pragma unroll
-        for (int o = 4; o < 32; o <<= 1)
-          l_s[bl][x] += __shfl_xor_sync(0xffffffffu, l_s[bl][x], o);
+      for (int o = 4; o < 32; o <<= 1)
+        l_s[x] += __shfl_xor_sync(0xffffffffu, l_s[x], o);
   };
   // A partial O is [column][dim]; padded columns are left out.  (In shared memory the
   // column stride and the order of the four stores keep a quarter-warp's banks apart.)
   auto store_part = [&](float* po, int stride, float4* ml, int cols) {
 #pragma unroll
-    for (int bl = 0; bl < kBlocks; ++bl)
+    for (int x = 0; x < 2; ++x) {
+      const int col = 2 * t + x;
+      if (col < cols) {
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const int col = bl * 8 + 2 * t + x;
-        if (col < cols) {
+        for (int i = 0; i < Cfg::kSteps; ++i) {
+          float4* dst = reinterpret_cast<float4*>(po + col * stride + part * Cfg::kDims +
+                                                  v_chunk(g, i) * 16);
+          const auto quad = [&](int y) {
+            return make_float4(acc[i * 8 + 2 * y][x], acc[i * 8 + 2 * y][2 + x],
+                               acc[i * 8 + 2 * y + 1][x],
+                               acc[i * 8 + 2 * y + 1][2 + x]);
+          };
 #pragma unroll
-          for (int i = 0; i < Cfg::kSteps; ++i) {
-            float4* dst = reinterpret_cast<float4*>(po + col * stride + part * Cfg::kDims +
-                                                    v_chunk(g, i) * 16);
-            const auto quad = [&](int y) {
-              return make_float4(acc[bl][i * 8 + 2 * y][x], acc[bl][i * 8 + 2 * y][2 + x],
-                                 acc[bl][i * 8 + 2 * y + 1][x],
-                                 acc[bl][i * 8 + 2 * y + 1][2 + x]);
-            };
-#pragma unroll
-            for (int y = 0; y < 4; ++y) dst[y ^ (g & 1)] = (g & 1) ? quad(y ^ 1) : quad(y);
-          }
-          if (g == 0 && part == 0)
-            ml[col] = make_float4(m_o[bl][x], m_s[bl][x], l_s[bl][x], 0.f);
+          for (int y = 0; y < 4; ++y) dst[y ^ (g & 1)] = (g & 1) ? quad(y ^ 1) : quad(y);
         }
+        if (g == 0 && part == 0)
+          ml[col] = make_float4(m_o[x], m_s[x], l_s[x], 0.f);
       }
+    }
   };
   auto finish = [&]() {  // the whole item lies in this run
 #pragma unroll
-    for (int bl = 0; bl < kBlocks; ++bl) {
+    for (int x = 0; x < 2; ++x) {
+      const int col = cg * kCols + 2 * t + x;
+      const float f = out_factor(m_o[x], m_s[x], l_s[x]);
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const int col = cg * kCols + bl * 8 + 2 * t + x;
-        const float f = out_factor(m_o[bl][x], m_s[bl][x], l_s[bl][x]);
+      for (int i = 0; i < Cfg::kSteps; ++i) {
+        float v[16];
 #pragma unroll
-        for (int i = 0; i < Cfg::kSteps; ++i) {
-          float v[16];
-#pragma unroll
-          for (int y = 0; y < 8; ++y) {
-            v[2 * y] = acc[bl][i * 8 + y][x];
-            v[2 * y + 1] = acc[bl][i * 8 + y][2 + x];
-          }
-          put_out(p, pl.b, head, col, part * Cfg::kDims + v_chunk(g, i) * 16, v, f);
+        for (int y = 0; y < 8; ++y) {
+          v[2 * y] = acc[i * 8 + y][x];
+          v[2 * y + 1] = acc[i * 8 + y][2 + x];
         }
-        if (g == 0 && part == 0) put_lse(p, pl.b, head, col, m_s[bl][x], l_s[bl][x]);
+        put_out(p, pl.b, head, col, part * Cfg::kDims + v_chunk(g, i) * 16, v, f);
       }
+      if (g == 0 && part == 0) put_lse(p, pl.b, head, col, m_s[x], l_s[x]);
     }
   };
 
   bool open = false;           // an item is in progress
   bool from_start = false;     // its first tile lies in this run
-  if (todo > 0) {
-    const RowPlan r = rows[pl.b];
-    from_start =
-        pl.left == (pl.item < heads * active_groups<kCols>(r, p.group) ? row_tiles(r) : 1);
-  }
+  if (todo > 0) from_start = list.at_start(pl);
 #pragma unroll 1
   while (todo > 0) {
     if (!open) {
@@ -571,7 +360,7 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1) kv8_attn_kernel(const Kv8Att
     // ---- S^T of the tile, through shared memory: rows g and g + 8 of both halves ----
     float k_scale[2];
     bool page_ok[2];
-    float* mine = exchange + (swap * Cfg::kWarps + warp) * (kBlocks * 256) + lane;
+    float* mine = exchange + (swap * Cfg::kWarps + warp) * 256 + lane;
 #pragma unroll 1
     for (int half = 0; half < 2; ++half) {
       asm volatile("cp.async.wait_group %0;" ::"n"(Cfg::kBufs - 1) : "memory");
@@ -583,11 +372,9 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1) kv8_attn_kernel(const Kv8Att
       page_ok[0] = half == 0 ? ok : page_ok[0];
       k_scale[1] = sc;
       page_ok[1] = ok;
-      float c[2][kBlocks][4];
+      float c[2][4];
 #pragma unroll
-      for (int bl = 0; bl < kBlocks; ++bl)
-#pragma unroll
-        for (int x = 0; x < 4; ++x) c[0][bl][x] = c[1][bl][x] = 0.f;
+      for (int x = 0; x < 4; ++x) c[0][x] = c[1][x] = 0.f;
       const uint8_t* r0 = kb + g * Cfg::kRow + 32 * t;
 #pragma unroll
       for (int i = 0; i < Cfg::kChunks; ++i) {
@@ -600,38 +387,32 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1) kv8_attn_kernel(const Kv8Att
           uint32_t a[4];
           kv8_to_half<kInt8>(xw[j], a[0], a[2]);
           kv8_to_half<kInt8>(yw[j], a[1], a[3]);
-#pragma unroll
-          for (int bl = 0; bl < kBlocks; ++bl)
-            mma_16816(c[kBlocks == 1 ? j & 1 : 0][bl], a, qf[bl][i][2 * j], qf[bl][i][2 * j + 1]);
+          mma_16816(c[j & 1], a, qf[i][2 * j], qf[i][2 * j + 1]);
         }
       }
 #pragma unroll
-      for (int bl = 0; bl < kBlocks; ++bl)
-#pragma unroll
-        for (int x = 0; x < 4; ++x)
-          mine[((half * kBlocks + bl) * 4 + x) * 32] =
-              kBlocks == 1 ? c[0][bl][x] + c[1][bl][x] : c[0][bl][x];
+      for (int x = 0; x < 4; ++x)
+        mine[(half * 4 + x) * 32] =
+            c[0][x] + c[1][x];
       __syncwarp();
       request();
       use = use + Cfg::kBuf == Cfg::kRing ? 0 : use + Cfg::kBuf;
     }
     if constexpr (kTeam > 1)
       asm volatile("bar.sync %0, %1;" ::"r"(1 + team), "n"(32 * kTeam) : "memory");
-    float s[2][kBlocks][4];
+    float s[2][4];
     {  // the team's partial sums, added in the same order by all
-      const float* all = exchange + (swap * Cfg::kWarps + team * kTeam) * (kBlocks * 256) + lane;
+      const float* all = exchange + (swap * Cfg::kWarps + team * kTeam) * 256 + lane;
 #pragma unroll
       for (int half = 0; half < 2; ++half)
 #pragma unroll
-        for (int bl = 0; bl < kBlocks; ++bl)
+        for (int x = 0; x < 4; ++x) {
+          const int at = (half * 4 + x) * 32;
+          float sum = all[at];
 #pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            const int at = ((half * kBlocks + bl) * 4 + x) * 32;
-            float sum = all[at];
-#pragma unroll
-            for (int w = 1; w < kTeam; ++w) sum += all[w * (kBlocks * 256) + at];
-            s[half][bl][x] = sum;
-          }
+          for (int w = 1; w < kTeam; ++w) sum += all[w * 256 + at];
+          s[half][x] = sum;
+        }
       if constexpr (kTeam > 1) swap ^= 1;
     }
 
@@ -647,91 +428,83 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1) kv8_attn_kernel(const Kv8Att
       v_exp[half] = static_cast<float>(e);
       v_mant[half] = e == -127 ? 0.f : __uint_as_float((bits & 0x807fffffu) | 0x3f800000u);
     }
-    uint32_t pf[2][kBlocks][2];  // P^T as B operands: column g, keys t, t + 4, t + 8, t + 12
+    uint32_t pf[2][2];  // P^T as B operands: column g, keys t, t + 4, t + 8, t + 12
     bool rescale = false;
-    float alpha[kBlocks][2];
+    float alpha[2];
     const int k_first = pl.tile * kKv8Tile + g;
+    uint32_t pk[2][2];         // [half][rows g, g + 8], columns 2t and 2t + 1
+    float pv[2][2][2];         // [column][half][row]
 #pragma unroll
-    for (int bl = 0; bl < kBlocks; ++bl) {
-      uint32_t pk[2][2];         // [half][rows g, g + 8], columns 2t and 2t + 1
-      float pv[2][2][2];         // [column][half][row]
+    for (int x = 0; x < 2; ++x) {
+      const int hi = last_key[x];
+      const int lo = p.window > 0 ? hi - p.window : -1;    // keys > lo are visible
+      float z[2][2];
 #pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        const int hi = last_key[bl][x];
-        const int lo = p.window > 0 ? hi - p.window : -1;    // keys > lo are visible
-        float z[2][2];
+      for (int half = 0; half < 2; ++half)
 #pragma unroll
-        for (int half = 0; half < 2; ++half)
-#pragma unroll
-          for (int y = 0; y < 2; ++y) {
-            const int k = k_first + half * 16 + y * 8;
-            z[half][y] = page_ok[half] && k <= hi && k > lo
-                             ? s[half][bl][2 * y + x] * (k_scale[half] * q_back[bl][x])
-                             : -INFINITY;
-          }
-        float top = fmaxf(z[0][0], z[0][1]), top1 = fmaxf(z[1][0], z[1][1]);
-        float top_v = fmaxf(top + v_exp[0], top1 + v_exp[1]);
-        top = fmaxf(top, top1);
-#pragma unroll
-        for (int o = 4; o < 32; o <<= 1) {
-          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-          top_v = fmaxf(top_v, __shfl_xor_sync(0xffffffffu, top_v, o));
+        for (int y = 0; y < 2; ++y) {
+          const int k = k_first + half * 16 + y * 8;
+          z[half][y] = page_ok[half] && k <= hi && k > lo
+                           ? s[half][2 * y + x] * (k_scale[half] * q_back[x])
+                           : -INFINITY;
         }
-        const float m_new = fmaxf(m_s[bl][x], top);
-        const float m_use = m_new == -INFINITY ? 0.f : m_new;
-        l_s[bl][x] = l_s[bl][x] * ex2(m_s[bl][x] - m_use) +
-                     ((ex2(z[0][0] - m_use) + ex2(z[0][1] - m_use)) +
-                      (ex2(z[1][0] - m_use) + ex2(z[1][1] - m_use)));
-        m_s[bl][x] = m_new;
-        alpha[bl][x] = 1.f;
-        if (top_v > m_o[bl][x] + kStale) {  // also the first visible key
-          alpha[bl][x] = m_o[bl][x] == -INFINITY ? 0.f : ex2(m_o[bl][x] - top_v);
-          m_o[bl][x] = top_v;
-          rescale = true;
-        }
-        const float m_sub = (m_o[bl][x] == -INFINITY ? 0.f : m_o[bl][x]) - kShiftUp;
+      float top = fmaxf(z[0][0], z[0][1]), top1 = fmaxf(z[1][0], z[1][1]);
+      float top_v = fmaxf(top + v_exp[0], top1 + v_exp[1]);
+      top = fmaxf(top, top1);
 #pragma unroll
-        for (int half = 0; half < 2; ++half)
-#pragma unroll
-          for (int y = 0; y < 2; ++y)
-            pv[x][half][y] = ex2(z[half][y] + v_exp[half] - m_sub) * v_mant[half];
+      for (int o = 4; o < 32; o <<= 1) {
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        top_v = fmaxf(top_v, __shfl_xor_sync(0xffffffffu, top_v, o));
       }
+      const float m_new = fmaxf(m_s[x], top);
+      const float m_use = m_new == -INFINITY ? 0.f : m_new;
+      l_s[x] = l_s[x] * ex2(m_s[x] - m_use) +
+                   ((ex2(z[0][0] - m_use) + ex2(z[0][1] - m_use)) +
+                    (ex2(z[1][0] - m_use) + ex2(z[1][1] - m_use)));
+      m_s[x] = m_new;
+      alpha[x] = 1.f;
+      if (top_v > m_o[x] + kStale) {  // also the first visible key
+        alpha[x] = m_o[x] == -INFINITY ? 0.f : ex2(m_o[x] - top_v);
+        m_o[x] = top_v;
+        rescale = true;
+      }
+      const float m_sub = (m_o[x] == -INFINITY ? 0.f : m_o[x]) - kShiftUp;
 #pragma unroll
-      for (int half = 0; half < 2; ++half) {
+      for (int half = 0; half < 2; ++half)
 #pragma unroll
-        for (int y = 0; y < 2; ++y) {
-          const __half2 v = __floats2half2_rn(pv[0][half][y], pv[1][half][y]);
-          pk[half][y] = *reinterpret_cast<const uint32_t*>(&v);
-        }
-        const uint32_t sel = (g & 1) ? 0x7632u : 0x5410u;
+        for (int y = 0; y < 2; ++y)
+          pv[x][half][y] = ex2(z[half][y] + v_exp[half] - m_sub) * v_mant[half];
+    }
 #pragma unroll
-        for (int y = 0; y < 2; ++y) {
-          const uint32_t x0 = __shfl_sync(0xffffffffu, pk[half][y], t * 4 + (g >> 1));
-          const uint32_t x1 = __shfl_sync(0xffffffffu, pk[half][y], (t + 4) * 4 + (g >> 1));
-          pf[half][bl][y] = __byte_perm(x0, x1, sel);
-        }
+    for (int half = 0; half < 2; ++half) {
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        const __half2 v = __floats2half2_rn(pv[0][half][y], pv[1][half][y]);
+        pk[half][y] = *reinterpret_cast<const uint32_t*>(&v);
+      }
+      const uint32_t sel = (g & 1) ? 0x7632u : 0x5410u;
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        const uint32_t x0 = __shfl_sync(0xffffffffu, pk[half][y], t * 4 + (g >> 1));
+        const uint32_t x1 = __shfl_sync(0xffffffffu, pk[half][y], (t + 4) * 4 + (g >> 1));
+        pf[half][y] = __byte_perm(x0, x1, sel);
       }
     }
     if (__any_sync(0xffffffffu, rescale)) {
 #pragma unroll
-      for (int bl = 0; bl < kBlocks; ++bl)
-#pragma unroll
-        for (int i = 0; i < Cfg::kTilesM; ++i) {
-          acc[bl][i][0] *= alpha[bl][0];
-          acc[bl][i][1] *= alpha[bl][1];
-          acc[bl][i][2] *= alpha[bl][0];
-          acc[bl][i][3] *= alpha[bl][1];
-        }
+      for (int i = 0; i < Cfg::kTilesM; ++i) {
+        acc[i][0] *= alpha[0];
+        acc[i][1] *= alpha[1];
+        acc[i][2] *= alpha[0];
+        acc[i][3] *= alpha[1];
+      }
     }
     // ---- O^T += V^T P^T ----
 #pragma unroll 1
     for (int half = 0; half < 2; ++half) {
-      uint32_t pb[kBlocks][2];
-#pragma unroll
-      for (int bl = 0; bl < kBlocks; ++bl) {
-        pb[bl][0] = half == 0 ? pf[0][bl][0] : pf[1][bl][0];
-        pb[bl][1] = half == 0 ? pf[0][bl][1] : pf[1][bl][1];
-      }
+      uint32_t pb[2];
+      pb[0] = half == 0 ? pf[0][0] : pf[1][0];
+      pb[1] = half == 0 ? pf[0][1] : pf[1][1];
       const uint8_t* r0 = ring + use + t * Cfg::kRow;
 #pragma unroll
       for (int i = 0; i < Cfg::kSteps; ++i) {
@@ -751,11 +524,8 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1) kv8_attn_kernel(const Kv8Att
           kv8_to_half<kInt8>(__byte_perm(w[2][y], w[3][y], 0x5140), a[2], a[3]);
           kv8_to_half<kInt8>(__byte_perm(w[0][y], w[1][y], 0x7362), c[0], c[1]);
           kv8_to_half<kInt8>(__byte_perm(w[2][y], w[3][y], 0x7362), c[2], c[3]);
-#pragma unroll
-          for (int bl = 0; bl < kBlocks; ++bl) {
-            mma_16816(acc[bl][i * 8 + 2 * y], a, pb[bl][0], pb[bl][1]);
-            mma_16816(acc[bl][i * 8 + 2 * y + 1], c, pb[bl][0], pb[bl][1]);
-          }
+          mma_16816(acc[i * 8 + 2 * y], a, pb[0], pb[1]);
+          mma_16816(acc[i * 8 + 2 * y + 1], c, pb[0], pb[1]);
         }
       }
       __syncwarp();
@@ -782,7 +552,7 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1) kv8_attn_kernel(const Kv8Att
       }
       if (!open) {
         from_start = true;
-        next_item(pl);
+        list.next_item(pl);
       }
     }
   }
@@ -828,7 +598,7 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1) kv8_attn_kernel(const Kv8Att
     const bool whole = tails[Cfg::kTeams + w0] && tails[2 * Cfg::kTeams + w1 - 1];
     const int b = tails[3 * Cfg::kTeams + w0];
     int h, grp;
-    item_head(b, key - b * (heads * p.col_groups), h, grp);
+    list.item_head(b, key - b * (heads * p.col_groups), h, grp);
     const int cols = min(kCols, p.rows.tokens * p.group - grp * kCols);
     const int64_t sl = 2 * (static_cast<int64_t>(blockIdx.x) * Cfg::kTeams + w0) + 1;
     for (int u = tid; u < cols * (D / 4); u += blockDim.x) {  // four dims of a column
@@ -859,7 +629,7 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1) kv8_attn_kernel(const Kv8Att
 // parts are read by many threads at once), 1 when most have two or three.
 template <int kSub, int kThreads, int kAhead>
 __global__ void __launch_bounds__(kThreads) kv8_merge_kernel(const Kv8AttnParams p, const int d,
-                                                        const int teams) {
+                                                             const int teams) {
   constexpr int kUnits = kThreads / kSub;
   __shared__ float4 sh_o[kSub][kUnits];
   __shared__ float4 sh_ml[kSub][kUnits];
@@ -874,7 +644,7 @@ __global__ void __launch_bounds__(kThreads) kv8_merge_kernel(const Kv8AttnParams
   const RowPlan r = {row4.x, row4.y, row4.z, row4.w};
   const int act = (r.n * p.group + p.cols - 1) / p.cols;
   if (grp >= act) return;  // padding: written by the run that met it
-  const int nt = row_tiles(r);
+  const int nt = row_tiles(r, p.tile);
   const int i0 = row_first + (h * act + grp) * nt, i1 = i0 + nt;
   const int w0 = run_of(i0, runs, total), w1 = run_of(i1 - 1, runs, total);
   if (w0 == w1) return;                                       // one run had it all
@@ -923,16 +693,15 @@ __global__ void __launch_bounds__(kThreads) kv8_merge_kernel(const Kv8AttnParams
 
 namespace {
 
-// The launch shapes.  One block of 8 columns (decode): 256 dims per warp, 12 warps
-// (170 registers).  More columns: three blocks at once and 128 dims per warp, 8
-// warps (255 registers).
+// 256 dims per warp (at head dim 512 two warps share a run), 12 warps (170 registers),
+// three 16-key pieces in flight per warp: 153 KB per SM.  8 rows of 16k-17k keys,
+// D = 512, e4m3: 99 us against 82 us for their bytes alone.  Measured and slower: 8 or
+// 10 warps, 16 warps of 128 registers, four pieces, pieces brought by TMA.
 template <int D>
-using OneBlock = AttnShape<D, D / 256, 1, 12, 3>;
-template <int D>
-using ThreeBlocks = AttnShape<D, D / 128, 3, 8, 8>;
-
+using Decode = AttnShape<D, D / 256, 12, 3>;
 template <typename Cfg, bool kInt8>
 int launch_attn(const Kv8AttnParams& p, int ctas, cudaStream_t stream) {
+  static_assert(Cfg::smem(kKv8MaxBatch) <= kKv8MaxSmem, "shared memory of the largest batch");
   const int smem = Cfg::smem(p.rows.batch);
   cudaError_t e = cudaFuncSetAttribute(kv8_attn_kernel<Cfg, kInt8>,
                                        cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
@@ -943,27 +712,22 @@ int launch_attn(const Kv8AttnParams& p, int ctas, cudaStream_t stream) {
 }
 template <typename Cfg>
 Kv8AttnShape shape_of() {
-  return {Cfg::kCols, Cfg::kTeams, Cfg::kOut};
+  return {Cfg::kCols, kKv8Tile, Cfg::kTeams, Cfg::kOut};
 }
 
 }  // namespace
 
 Kv8AttnShape kv8_attn_shape(int d, int64_t columns) {
-  if (columns <= 8) return d == 512 ? shape_of<OneBlock<512>>() : shape_of<OneBlock<256>>();
-  return d == 512 ? shape_of<ThreeBlocks<512>>() : shape_of<ThreeBlocks<256>>();
+  if (columns > 8) return kv8_wide_shape(d, columns);
+  return d == 512 ? shape_of<Decode<512>>() : shape_of<Decode<256>>();
 }
 
 int launch_kv8_attn(int d, bool int8, const Kv8AttnParams& p, int ctas, cudaStream_t stream) {
-  if (p.cols == 8) {
-    if (d == 512) return int8 ? launch_attn<OneBlock<512>, true>(p, ctas, stream)
-                              : launch_attn<OneBlock<512>, false>(p, ctas, stream);
-    return int8 ? launch_attn<OneBlock<256>, true>(p, ctas, stream)
-                : launch_attn<OneBlock<256>, false>(p, ctas, stream);
-  }
-  if (d == 512) return int8 ? launch_attn<ThreeBlocks<512>, true>(p, ctas, stream)
-                            : launch_attn<ThreeBlocks<512>, false>(p, ctas, stream);
-  return int8 ? launch_attn<ThreeBlocks<256>, true>(p, ctas, stream)
-              : launch_attn<ThreeBlocks<256>, false>(p, ctas, stream);
+  if (p.cols > 8) return launch_kv8_wide(d, int8, p, ctas, stream);
+  if (d == 512) return int8 ? launch_attn<Decode<512>, true>(p, ctas, stream)
+                            : launch_attn<Decode<512>, false>(p, ctas, stream);
+  return int8 ? launch_attn<Decode<256>, true>(p, ctas, stream)
+              : launch_attn<Decode<256>, false>(p, ctas, stream);
 }
 
 int launch_kv8_merge(int d, const Kv8AttnParams& p, int ctas, cudaStream_t stream) {

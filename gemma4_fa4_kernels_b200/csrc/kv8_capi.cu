@@ -55,6 +55,8 @@ int check_cache(const g4_kv8_args* a) {
   if (a->num_kv_heads > 65535) return api_fail(G4_ERR_UNSUPPORTED, "too many KV heads");
   if (static_cast<int64_t>(a->pages_per_slot) * a->page_size > INT32_MAX - 65536)
     return api_fail(G4_ERR_UNSUPPORTED, "a sequence's positions must fit 31 bits");
+  if (static_cast<int64_t>(a->num_pages) * a->num_kv_heads * a->page_size > INT32_MAX)
+    return api_fail(G4_ERR_UNSUPPORTED, "a pool's (page, head, token) rows must fit 31 bits");
   if (!a->starts || !a->ends) return api_fail(G4_ERR_INVALID, "starts and ends are required");
   if (a->batch <= 0 || a->tokens <= 0)
     return api_fail(G4_ERR_INVALID, "batch and tokens must be positive");
@@ -112,7 +114,7 @@ int check_attn_shape(const g4_kv8_args* a) {
 // Launch shape and workspace of the attention.
 struct AttnPlan {
   int64_t tiles = 0;  // upper bound of the tile list
-  int cols = 0, col_groups = 0;
+  int cols = 0, tile = 0, col_groups = 0;
   int ctas = 0;
   size_t part_o = 0, part_ml = 0, plan = 0, total = 0;
 };
@@ -122,11 +124,12 @@ AttnPlan attn_plan(const g4_kv8_args* a) {
   const int64_t columns = int64_t(a->num_q_heads / a->num_kv_heads) * a->tokens;
   const Kv8AttnShape shape = kv8_attn_shape(a->head_dim, columns);
   w.cols = shape.cols;
+  w.tile = shape.tile;
   w.col_groups = static_cast<int>(
       std::min<int64_t>((columns + shape.cols - 1) / shape.cols, INT32_MAX));
   int64_t keys = a->max_seqlen_k;
   if (a->window > 0) keys = std::min<int64_t>(keys, int64_t(a->window) + a->tokens - 1);
-  const int64_t per_item = (keys + kKv8Tile - 1) / kKv8Tile + 1;
+  const int64_t per_item = (keys + shape.tile - 1) / shape.tile + 1;
   w.tiles = int64_t(a->batch) * a->num_kv_heads * w.col_groups * per_item;
   // one CTA per SM; fewer when there is less than a tile per run
   w.ctas = static_cast<int>(std::max<int64_t>(
@@ -317,6 +320,7 @@ int g4_kv8_attn(const g4_kv8_args* a, void* stream) {
   p.max_k = a->max_seqlen_k;
   p.group = a->num_q_heads / a->num_kv_heads;
   p.cols = w.cols;
+  p.tile = w.tile;
   p.col_groups = w.col_groups;
   p.q = static_cast<const __nv_bfloat16*>(a->q);
   p.o = static_cast<__nv_bfloat16*>(a->o);
@@ -328,6 +332,7 @@ int g4_kv8_attn(const g4_kv8_args* a, void* stream) {
   p.lse_stride[0] = a->lse_stride[0];
   p.lse_stride[1] = a->lse_stride[1];
   uint8_t* ws = static_cast<uint8_t*>(a->workspace);
+  p.status = a->status;
   p.plan = reinterpret_cast<int*>(ws + w.plan);
   p.part_ml = reinterpret_cast<float4*>(ws + w.part_ml);
   p.part_o = reinterpret_cast<float*>(ws + w.part_o);

@@ -455,6 +455,7 @@ class PagedKVCache8:
                 (_lib.G4_PAGES_EXHAUSTED, "no free page was left"),
                 (_lib.G4_PAGES_ROW_FULL, "a slot's table was full"),
                 (_lib.G4_PAGES_BAD_INDEX, "a slot, page or count was out of range or listed twice"),
+                (_lib.G4_KV8_DEVICE_WAIT, "a kernel's bounded wait expired (invalid results)"),
             ) if bits & bit]
             raise RuntimeError("paged cache: " + "; ".join(what))
 

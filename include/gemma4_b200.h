@@ -368,7 +368,7 @@ typedef struct g4_kv8_args {
   const int32_t* slots; /* nullable */
   const int32_t* starts;
   const int32_t* ends;
-  int32_t* status;      /* append, nullable: device word, G4_PAGES_* bits are or-ed in */
+  int32_t* status;      /* nullable: device word, G4_PAGES_* bits are or-ed in */
   /* append: inputs; read: outputs; [batch][token][kv head][head_dim] bf16 */
   void* k;
   void* v;
@@ -436,6 +436,7 @@ int g4_kv8_pad_rows(const g4_kv8_args* args, void* stream);
 #define G4_PAGES_EXHAUSTED 1
 #define G4_PAGES_ROW_FULL 2
 #define G4_PAGES_BAD_INDEX 4
+#define G4_KV8_DEVICE_WAIT 8 /* g4_kv8_attn: a bounded wait expired, its results are invalid */
 typedef struct g4_pages_args {
   int32_t* tables;
   int32_t* lengths;

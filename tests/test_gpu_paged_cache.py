@@ -86,7 +86,7 @@ class Pair:
         return starts, ends
 
 
-def bounds(out, lse, spread, grain, size, d, p_bits):
+def bounds(out, lse, spread, grain, size, d, p_bits, p_step):
     """Largest errors of O and LSE.
 
     S: d products summed in fp32, at most d/16 + 3 rounded (or truncated: 2^-23)
@@ -95,12 +95,13 @@ def bounds(out, lse, spread, grain, size, d, p_bits):
     rounded to 2^-24 of a few hundred at most (2^-15).  P is rounded to p_bits
     significant bits, and all of these move O by at most twice (numerator and
     denominator) their share of sum p |v|.  O itself is rounded to bf16: 2^-8 of it,
-    plus the smallest bf16 step.  The decode kernel holds 2^11 s_v P in fp16 relative
-    to its maximum, whose steps do not shrink below 2^-24: half a step is 2^-36 of the
-    largest s_v P, for every key, which grain = max(p s_v) sum |v8| adds up."""
+    plus the smallest bf16 step.  The kernels hold 2^11 s_v P (more than 8 columns:
+    2^5 s_v P) in fp16 relative to its maximum, whose steps do not shrink below 2^-24:
+    half a step is 2^-36 (2^-30) of the largest s_v P, for every key, which grain =
+    max(p s_v) sum |v8| adds up."""
     ds = (d / 16 + 7) * 2.0 ** -23 * size + 2.0 ** -15
     o = 2.0 ** -8 * np.abs(out) + (2.0 ** -p_bits + 2 * ds.transpose(0, 2, 1)[..., None]) * spread
-    o = o + 2.0 ** -36 * grain
+    o = o + p_step * grain
     return o + 2.0 ** -126, ds + 2.0 ** -21 * np.abs(np.where(np.isfinite(lse), lse, 0))
 
 
@@ -115,7 +116,8 @@ def check_attention(pair, layer, q, slots, starts, ends, **kw):
     d, group = dq.shape[3], dq.shape[2] // pair.ref.k.shape[2]
     direct = dq.shape[1] * group <= DIRECT_COLUMNS
     # the chunk path holds K and V (when scales are no powers of two) and P in bf16
-    o_tol, l_tol = bounds(out, lse, spread, grain, size, d, 11 if direct else 7)
+    o_tol, l_tol = bounds(out, lse, spread, grain, size, d, 11 if direct else 7,
+                          2.0 ** -36 if dq.shape[1] * group <= 8 else 2.0 ** -30)
     got, got_lse = f64(got), f64(got_lse)
     assert np.array_equal(np.isneginf(got_lse), np.isneginf(lse)), "masked rows differ"
     fin = np.isfinite(lse)
