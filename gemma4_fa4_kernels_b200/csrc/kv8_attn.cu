@@ -694,8 +694,8 @@ __global__ void __launch_bounds__(kThreads) kv8_merge_kernel(const Kv8AttnParams
 namespace {
 
 // 256 dims per warp (at head dim 512 two warps share a run), 12 warps (170 registers),
-// three 16-key pieces in flight per warp: 153 KB per SM.  8 rows of 16k-17k keys,
-// D = 512, e4m3: 99 us against 82 us for their bytes alone.  Measured and slower: 8 or
+// three 16-key pieces in flight per warp: 153 KB per SM.  One row of 131072 keys, 4 KV
+// heads, D = 512, e4m3: 99 us against 82 us for its bytes alone.  Measured and slower: 8 or
 // 10 warps, 16 warps of 128 registers, four pieces, pieces brought by TMA.
 template <int D>
 using Decode = AttnShape<D, D / 256, 12, 3>;

@@ -12,7 +12,7 @@
 // swizzle), which the MMA reads once: 4 bytes of shared-memory traffic per code, at
 // 128 bytes per clock 32 codes per clock and SM, against the SM's share of HBM of 23;
 // in practice the converters' issue slots and the waits between tiles.  Five drafted
-// tokens of 8 heads (40 columns) over 16 rows of 2k-4k int8 keys: 57 us with 14 us for
+// tokens of 8 heads (40 columns) over 6 rows of 700 to 9001 int8 keys: 57 us with 14 us for
 // the merge behind it, 94 and 12 with three blocks of 8 columns per pass of mma.sync.
 //
 // Warp roles: 8 softmax warps (two per 32 TMEM lanes, thread = key, half of the columns
@@ -40,10 +40,12 @@ constexpr int kSoft = 8;           // softmax warps
 constexpr int kFeeds = 3;          // pairs of converter warps
 constexpr int kConvWarps = 2 * kFeeds;
 constexpr int kWideThreads = (kSoft + 1 + kConvWarps) * 32;
-// s_v P in fp16 relative to O's reference: a reference that may lag by 2^9 and a shift
-// of 2^5 keep it below 2^14 (normal down to 2^-19 of the largest, steps of 2^-30 of it
-// below) and renewals, which cost as much as the rest of a tile, rare.
-constexpr float kWideShift = 5.f;
+// s_v P in fp16 relative to O's reference, whose s_v counts as the power of two above
+// it: a reference that may lag by 2^9 and a shift of 2^6 keep P below 2^15; its largest
+// is at least 2^5, so half a step is 2^-12 of a weight, or 2^-30 of the largest for
+// weights more than 2^19 below it.  Renewals, which cost as much as the rest of a tile,
+// stay rare.
+constexpr float kWideShift = 6.f;
 constexpr float kWideStale = 9.f;
 constexpr float kStaleSum = 8.f;   // log2 by which the row sum's reference may lag
 constexpr float kNoKey = -1e30f;   // reference before the first visible key: any score exceeds it
@@ -493,7 +495,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv8_wide_kernel(const Kv8Attn
                           __all_sync(0xffffffffu, key_ok);
         const float v_exp =
             static_cast<float>(static_cast<int>((__float_as_uint(vs) >> 23) & 255u) - 126);
-        const float vs_up = vs * 32.f;  // 2^kWideShift
+        const float vs_up = vs * 64.f;  // 2^kWideShift
         if (ok) ok = mbar_wait(&misc->s_full[b], (tile >> 1) & 1, ab, kDevTimeoutMma);
         ok = __all_sync(0xffffffffu, ok);
         tc_fence_after();

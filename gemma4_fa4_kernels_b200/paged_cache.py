@@ -50,10 +50,13 @@ PAGE_SIZES = (16, 32, 64, 128)
 CODE_DTYPES = {torch.float8_e4m3fn: _lib.G4_KV8_E4M3, torch.int8: _lib.G4_KV8_INT8}
 MAX_ROWS = 1024
 
-# Up to this many (token, query head) columns per KV head and row the queries read
-# the codes directly; longer chunks of prompts run the tensor-core forward over a
-# BF16 copy of the keys they see.
-DIRECT_COLUMNS = 128
+# Up to this many (token, query head) columns per KV head and row, by head dim, the
+# queries read the codes directly; longer chunks of prompts run the tensor-core forward
+# over a BF16 copy of the keys they see.  Measured, us, direct against copy (1 and 4 rows):
+#   d512, 1500 keys     256 columns  69 / 63,   73 / 81    512 columns   52 / 65,  120 / 83
+#   d512, 17000 keys    256 columns 155 / 417, 386 / 587   512 columns  208 / 421, 724 / 589
+#   d256, window 1024    32 columns  30 / 37,   36 / 50     64 columns   42 / 36,   54 / 52
+DIRECT_COLUMNS = {512: 256, 256: 32}
 
 
 def _strides(t: torch.Tensor) -> list[int]:
@@ -342,7 +345,7 @@ class PagedKVCache8:
             raise ValueError("q strides must be positive multiples of 8 elements")
         if not batch or not tokens:
             return self._keep(key, (batch, None, (batch, heads, tokens), 0, False))
-        chunk = tokens * (heads // self.num_kv_heads) > DIRECT_COLUMNS
+        chunk = tokens * (heads // self.num_kv_heads) > DIRECT_COLUMNS[d]
         if chunk:  # LSE as the packed forward writes it: (head, row, token)
             a.lse_stride[:] = (tokens, batch * tokens)
             ws_bytes = 0

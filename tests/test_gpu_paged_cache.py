@@ -114,7 +114,7 @@ def check_attention(pair, layer, q, slots, starts, ends, **kw):
     assert got.shape == dq.shape and got.dtype == torch.bfloat16
     assert got_lse.shape == (dq.shape[0], dq.shape[2], dq.shape[1])
     d, group = dq.shape[3], dq.shape[2] // pair.ref.k.shape[2]
-    direct = dq.shape[1] * group <= DIRECT_COLUMNS
+    direct = dq.shape[1] * group <= DIRECT_COLUMNS[d]
     # the chunk path holds K and V (when scales are no powers of two) and P in bf16
     o_tol, l_tol = bounds(out, lse, spread, grain, size, d, 11 if direct else 7,
                           2.0 ** -36 if dq.shape[1] * group <= 8 else 2.0 ** -30)
@@ -336,11 +336,84 @@ def test_attention_is_repeatable_and_reads_strided_queries():
 
 
 @pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("d,heads,group,tokens,page,window,lens", [
+    (512, 1, 8, 4, 64, 0, [900, 128, 129, 4]),          # 32 columns, all of them used
+    (512, 2, 8, 5, 16, 300, [700, 40, 301, 300, 5]),    # 40 of 64, pages inside a tile
+    (512, 1, 3, 11, 128, 0, [1500, 11]),                # 33 of 64
+    (512, 1, 8, 32, 32, 0, [400, 33, 1000]),            # four groups of 64 columns
+    (512, 1, 8, 17, 32, 100, [17, 600]),                # 64, 64 and 8
+    (256, 2, 2, 12, 32, 1024, [2500, 12, 130, 1100]),   # 24 of 32
+    (256, 3, 16, 2, 64, 0, [2, 1000]),                  # 32, few keys and many
+    (256, 16, 2, 5, 16, 64, [70] * 40),                 # many items per CTA
+])
+def test_wide_shapes(fmt, d, heads, group, tokens, page, window, lens):
+    """More than 8 columns: every launch shape, groups of columns, windows, padding."""
+    rng = np.random.default_rng(tokens + len(lens))
+    p = Pair(fmt, heads=heads, d=d, page=page, pages=2 + sum(-(-x // page) for x in lens),
+             slots=len(lens), per_slot=-(-max(lens) // page))
+    rows = list(range(len(lens)))
+    p.fill(rows, lens, rng)
+    n = [tokens - (b % 3 if b else 0) for b in rows]
+    q = 0.3 * rng.standard_normal((len(lens), tokens, heads * group, d))
+    check_attention(p, 0, q, rows, [e - m for e, m in zip(lens, n)], lens, window=window)
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("d,group,tokens", [(512, 8, 2), (512, 8, 6), (256, 4, 8)])
+def test_wide_maxima_that_rise_and_scales_of_any_size(fmt, d, group, tokens):
+    """Scores that grow along the keys, so that every tile renews the references, with
+    V scales that differ by many powers of two and queries of very different size."""
+    rng = np.random.default_rng(d + tokens)
+    n, page = 1000, 16
+    p = Pair(fmt, heads=1, d=d, page=page, pages=66, slots=1, per_slot=64)
+    p.extend([0], [n])
+    u = rng.standard_normal(d)
+    u /= np.linalg.norm(u)
+    k = rng.standard_normal((1, n, 1, d)) + (np.arange(n) / 8.0)[None, :, None, None] * u
+    v = rng.standard_normal((1, n, 1, d))
+    p.append(0, k, v, [0], [0], [n])
+    p.ref.v_scale[:] = 2.0 ** rng.integers(-40, 40, p.ref.v_scale.shape)
+    p.ref.v_scale[0, 5, 0] = 1.37
+    p.dev.v_scale.copy_(torch.tensor(p.ref.v_scale))
+    p.ref.v_scale[:] = f64(p.dev.v_scale)
+    size = np.array([1e-30, 1e-3, 0.2, 1.0])[np.arange(group) % 4][:, None]
+    q = size * (u + 0.02 * rng.standard_normal((1, tokens, group, d)))
+    check_attention(p, 0, q, [0], [n - tokens], [n])
+
+
+def test_wide_empty_rows_masked_pages_and_stale_slots():
+    rng = np.random.default_rng(21)
+    p = Pair("e4m3", heads=1, d=512, page=16, pages=40, slots=8, per_slot=20)
+    lens = [250, 37, 50, 20, 6]
+    p.fill([0, 1, 2, 3, 4], lens, rng)
+    codes = p.dev.k.view(torch.uint8), p.dev.v.view(torch.uint8)
+    for page in np.flatnonzero(p.ref.refcounts == 0):
+        for c in codes:
+            c[:, page] = 0x7F
+        p.dev.k_scale[:, page] = float("nan")
+        p.dev.v_scale[:, page] = float("inf")
+    for slot, n in enumerate(lens):
+        if n % 16:
+            for c in codes:
+                c[:, int(p.ref.tables[slot, (n - 1) // 16]), :, n % 16:] = 0x7F
+    p.ref.tables[0, 3] = p.ref.tables[1, 1] = -1   # holes, a row of them, a bad id
+    p.ref.tables[0, 8:16] = -1                     # a whole tile
+    p.ref.tables[2, :] = -1
+    p.ref.tables[3, 0] = 40
+    p.dev.tables.copy_(i32(p.ref.tables))
+    q = 0.3 * rng.standard_normal((9, 5, 8, 512))
+    check_attention(p, 0, q, [0, 1, 2, 3, 4, 5, 9, -2, 0], [245, 35, 45, 18, 1, 0, 3, 3, 318],
+                    [250, 37, 50, 20, 6, 0, 5, 5, 321])
+    got = check_attention(p, 0, q[:2], [0, 1], [246, 35], [250, 37], max_seqlen_k=249)
+    assert not got[0].any() and got[1].any()
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
 @pytest.mark.parametrize("d,heads,group,window", [(512, 1, 8, 0), (256, 2, 2, 0), (256, 2, 2, 50)])
 def test_chunks_of_prompts(fmt, d, heads, group, window):
     """More queries than the direct kernel takes: ragged, padded and empty rows."""
     rng = np.random.default_rng(14)
-    tokens = DIRECT_COLUMNS // group + 3
+    tokens = DIRECT_COLUMNS[d] // group + 3
     lens = [tokens, tokens + 90, 200, 5]
     p = Pair(fmt, heads=heads, d=d, page=64, pages=30, slots=5, per_slot=6)
     p.fill([0, 1, 2, 3], lens, rng)

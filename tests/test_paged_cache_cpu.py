@@ -177,6 +177,13 @@ def test_strides_must_be_16_byte_multiples():
     assert "multiples of 8" in _lib.last_error()
 
 
+def test_pools_of_more_than_31_bits_of_rows_are_refused():
+    for fn in ("g4_kv8_append", "g4_kv8_read", "g4_kv8_attn"):
+        a = _kv8(num_pages=1 << 25, page_size=16)
+        assert getattr(_lib.load(), fn)(ctypes.byref(a), None) == _lib.G4_ERR_UNSUPPORTED
+        assert "rows must fit 31 bits" in _lib.last_error()
+
+
 def test_chunk_plan_refuses_rows_past_31_bits():
     a = _kv8(batch=1024, tokens=1 << 22)
     rc = _lib.load().g4_kv8_chunk_plan(ctypes.byref(a), 16, 32, 48, 64, None)
