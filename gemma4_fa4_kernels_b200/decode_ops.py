@@ -1,4 +1,4 @@
-"""Single-token static-cache decode layer ops for Gemma-4 (B=1, Q=1).
+"""Decode layer ops for Gemma-4: static caches (B=1, Q=1) and the paged 8-bit cache.
 
 The opaque operators of the reference's compiled decode path
 (src/gemma4_fa4/h100_torch_ops.py:479-880, registered at :1007-1017): one
@@ -23,6 +23,13 @@ its packed forward, both of which equal this single-row lower-right result.
 Projections are plain cuBLAS BF16 GEMMs (``torch.nn.functional.linear``); the
 Q/K norms, the rotary embedding and the value norm run in the fused
 ``g4_prep_fwd`` kernel (global layers: K and V from one read of Z).
+
+:func:`global_paged_cache_decode_fwd` and :func:`local_paged_cache_decode_fwd` are
+the same layers over a :class:`~gemma4_fa4_kernels_b200.PagedKVCache8`: a batch of
+sequences of any lengths, one or several (drafted) tokens or a chunk of a prompt
+each, the new K and V appended as 8-bit codes.  Lengths and tables stay on the
+device, so these calls never wait for it and can be captured into a graph; the
+cache is an object, so they are plain functions and not custom ops.
 """
 
 from __future__ import annotations
@@ -31,6 +38,7 @@ import torch
 
 from . import ops
 from .errors import UnsupportedB200Path
+from .paged_cache import PagedKVCache8
 from .prep import prep_fwd
 
 HIDDEN_SIZE = 5376
@@ -199,14 +207,14 @@ local_static_cache_decode_op = torch.library.custom_op(
 torch.library.register_fake(LOCAL_STATIC_CACHE_DECODE_OP_NAME)(_fake)
 
 
-def _check_call_boundary(hidden_states, cos, sin) -> None:
+def _check_call_boundary(hidden_states, cos, sin, kind="static-cache") -> None:
     """Reject autograd before the custom op disables grad mode for its body."""
     if torch.is_grad_enabled():
-        raise UnsupportedB200Path("static-cache decode ops require inference / no-grad mode")
+        raise UnsupportedB200Path(f"{kind} decode ops require inference / no-grad mode")
     names = [n for n, t in zip(("hidden_states", "cos", "sin"), (hidden_states, cos, sin))
              if t.requires_grad]
     if names:
-        raise UnsupportedB200Path("static-cache decode ops reject requires_grad activations: "
+        raise UnsupportedB200Path(f"{kind} decode ops reject requires_grad activations: "
                                   + ", ".join(names))
 
 
@@ -230,3 +238,73 @@ def local_static_cache_decode_fwd(hidden_states, cos, sin, position_ids, cache_k
     return local_static_cache_decode_op(hidden_states, cos, sin, position_ids, cache_k, cache_v,
                                         cache_length, q_proj_weight, k_proj_weight, v_proj_weight,
                                         o_proj_weight, q_norm_weight, k_norm_weight)
+
+
+# ------------------------------------------------------------------------------------
+# layers over the paged 8-bit cache
+# ------------------------------------------------------------------------------------
+def _paged_layer(label, geometry, window, cache, layer, hidden_states, cos, sin, slots, starts,
+                 ends, q_proj_weight, k_proj_weight, v_proj_weight, o_proj_weight, q_norm_weight,
+                 k_norm_weight, max_seqlen_k):
+    _check_call_boundary(hidden_states, cos, sin, "paged-cache")
+    hq, hkv, d = geometry
+    if not isinstance(cache, PagedKVCache8):
+        raise ValueError(f"{label} decode requires a PagedKVCache8")
+    if (cache.num_kv_heads, cache.head_dim) != (hkv, d):
+        raise UnsupportedB200Path(f"{label} decode requires a cache of {hkv} KV heads of {d}")
+    weights = [w for w in (q_proj_weight, k_proj_weight, v_proj_weight, o_proj_weight,
+                           q_norm_weight, k_norm_weight) if w is not None]
+    if hidden_states.ndim != 3 or hidden_states.shape[2] != HIDDEN_SIZE:
+        raise UnsupportedB200Path(f"{label} decode hidden states must be (rows, tokens, "
+                                  f"{HIDDEN_SIZE})")
+    rows, tokens = hidden_states.shape[:2]
+    if cos.shape != (rows, tokens, d) or sin.shape != cos.shape:
+        raise ValueError(f"{label} decode rotary tensors must be ({rows}, {tokens}, {d})")
+    _check_weights(label, weights, [(hq * d, HIDDEN_SIZE), (hkv * d, HIDDEN_SIZE)]
+                   + [(hkv * d, HIDDEN_SIZE)] * (v_proj_weight is not None)
+                   + [(HIDDEN_SIZE, hq * d), (d,), (d,)])
+    if any(t.dtype != torch.bfloat16 for t in (hidden_states, cos, sin, *weights)):
+        raise ValueError(f"{label} decode activations and weights must be BF16")
+    if any(t.device != cache.device for t in (hidden_states, cos, sin, *weights)):
+        raise ValueError(f"{label} decode tensors must be on the cache's device ({cache.device})")
+    lin = torch.nn.functional.linear
+    with torch.cuda.device(cache.device):
+        q, _ = prep_fwd(lin(hidden_states, q_proj_weight).view(rows, tokens, hq, d),
+                        q_norm_weight, cos, sin, d)
+        k, v = prep_fwd(lin(hidden_states, k_proj_weight).view(rows, tokens, hkv, d),
+                        k_norm_weight, cos, sin, d, want_plain=v_proj_weight is None)
+        if v_proj_weight is not None:
+            _, v = prep_fwd(lin(hidden_states, v_proj_weight).view(rows, tokens, hkv, d), None,
+                            None, None, 0, want_rot=False, want_plain=True)
+        cache.append(layer, k, v, slots, starts, ends)
+        attn, lse = cache.attention(layer, q, slots, starts, ends, window=window,
+                                    max_seqlen_k=max_seqlen_k)
+        return lin(attn.view(rows, tokens, hq * d), o_proj_weight), lse
+
+
+def global_paged_cache_decode_fwd(cache, layer, hidden_states, cos, sin, slots, starts, ends,
+                                  q_proj_weight, k_proj_weight, o_proj_weight, q_norm_weight,
+                                  k_norm_weight, *, max_seqlen_k=None):
+    """One global layer over ``layer`` of a paged cache: the tokens at positions
+    ``starts .. ends - 1`` (:meth:`PagedKVCache8.extend`) of each row are appended and
+    attend over their sequence up to themselves.
+
+    ``hidden_states`` (rows, tokens, 5376) and the rotary tables of the tokens'
+    positions (rows, tokens, 512) are padded: row b uses its first ``ends - starts``
+    tokens.  Returns ``(out (rows, tokens, 5376) BF16, lse (rows, 32, tokens) FP32)``;
+    padding gives zeros and -inf."""
+    return _paged_layer("global paged-cache", GLOBAL_GEOMETRY, 0, cache, layer, hidden_states,
+                        cos, sin, slots, starts, ends, q_proj_weight, k_proj_weight, None,
+                        o_proj_weight, q_norm_weight, k_norm_weight, max_seqlen_k)
+
+
+def local_paged_cache_decode_fwd(cache, layer, hidden_states, cos, sin, slots, starts, ends,
+                                 q_proj_weight, k_proj_weight, v_proj_weight, o_proj_weight,
+                                 q_norm_weight, k_norm_weight, *, max_seqlen_k=None):
+    """One local layer (window 1024) over ``layer`` of a paged cache, as
+    :func:`global_paged_cache_decode_fwd`; rotary tables are (rows, tokens, 256).
+    Pages that the window left go back with :meth:`PagedKVCache8.trim`."""
+    return _paged_layer("local paged-cache", LOCAL_GEOMETRY, LOCAL_WINDOW, cache, layer,
+                        hidden_states, cos, sin, slots, starts, ends, q_proj_weight,
+                        k_proj_weight, v_proj_weight, o_proj_weight, q_norm_weight,
+                        k_norm_weight, max_seqlen_k)
