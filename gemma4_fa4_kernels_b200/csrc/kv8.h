@@ -121,6 +121,7 @@ struct Kv8AttnParams {
   int cols;                 // (token, query head) columns of one item (Kv8AttnShape)
   int tile;                 // keys per tile of the list
   int col_groups;           // ceil(tokens * group / cols)
+  bool whole;               // one CTA per item instead of equal runs: nothing to merge
   const __nv_bfloat16* q;   // (batch, token, head) strides in elements
   int64_t q_stride[3];
   __nv_bfloat16* o;
@@ -131,7 +132,7 @@ struct Kv8AttnParams {
   float* part_o;            // [slot][cols][head_dim]
   float4* part_ml;          // [slot][cols]: (shift of O, max, sum, -)
   int* status;              // nullable
-  int* plan;                // {runs, tiles, -, -}, the rows' plans (int4 each), their first tiles
+  int* plan;                // (not used if whole) {runs, tiles, -, -}, the rows' plans (int4 each), their first tiles
 };
 // The kernel's launch shape for a row's number of (token, query head) columns.
 struct Kv8AttnShape {

@@ -128,17 +128,34 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1) kv8_attn_kernel(const Kv8Att
   const int B = p.rows.batch, heads = p.cache.heads;
   const auto row_at = [&](int b) { return rows[b]; };
   const TileList<kKv8Tile, kCols, decltype(row_at)> list{p, row_at, prefix};
-  plan_rows<Cfg::kThreads>(p, list, prefix, scan, [&](int b, const RowPlan& r) { rows[b] = r; });
-  const int total = prefix[B];
-  const int runs = min(total, static_cast<int>(gridDim.x) * Cfg::kTeams);
-  if (blockIdx.x == 0 && tid == 0)
-    *reinterpret_cast<int4*>(p.plan) = make_int4(runs, total, 0, 0);
   const int W = blockIdx.x * Cfg::kTeams + team;
-  const int w_begin = W < runs ? run_begin(W, runs, total) : 0;
-  int todo = W < runs ? run_begin(W + 1, runs, total) - w_begin : 0;
+  Place first;
+  int todo = 0;
+  if (p.whole) {  // the CTA's item, cut into a run per team
+    const int items = heads * p.col_groups, b = blockIdx.x / items;
+    if (tid == 0) rows[b] = row_plan(p, b);
+    __syncthreads();
+    first = list.item_place(b, blockIdx.x - b * items);
+    const int runs = min(first.left, Cfg::kTeams);
+    if (team < runs) {
+      const int at = run_begin(team, runs, first.left);
+      todo = run_begin(team + 1, runs, first.left) - at;
+      first.tile += at;
+      first.left -= at;
+    }
+  } else {
+    plan_rows<Cfg::kThreads>(p, list, prefix, scan, [&](int b, const RowPlan& r) { rows[b] = r; });
+    const int total = prefix[B];
+    const int runs = min(total, static_cast<int>(gridDim.x) * Cfg::kTeams);
+    if (blockIdx.x == 0 && tid == 0)
+      *reinterpret_cast<int4*>(p.plan) = make_int4(runs, total, 0, 0);
+    const int begin = W < runs ? run_begin(W, runs, total) : 0;
+    if (W < runs) todo = run_begin(W + 1, runs, total) - begin;
+    first = list.locate(begin);
+  }
 
   // ---- the loading side: 16-key pieces in order K0a K0b V0a V0b K1a ... ----
-  Place ld = list.locate(w_begin);
+  Place ld = first;
   int ld_todo = todo;        // tiles not yet requested
   uint32_t ld_buf = 0;       // ring offset of the next request
   int ld_phase = 0;          // 0, 1: K halves; 2, 3: V halves
@@ -229,7 +246,7 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1) kv8_attn_kernel(const Kv8Att
   float m_o[2], m_s[2], l_s[2];           // columns 2t, 2t + 1: shift of O; max and sum of P
   float q_back[2];               // log2(e) * 2^-e of the column's Q
   int last_key[2];               // last visible key, -1: a padded column
-  Place pl = list.locate(w_begin);
+  Place pl = first;
   uint32_t use = 0;                       // ring offset of the next piece
   int head = 0, cg = 0, swap = 0;
 

@@ -111,11 +111,19 @@ int check_attn_shape(const g4_kv8_args* a) {
   return G4_OK;
 }
 
+// A call of at most one item per SM gives each item a CTA when that is at most this many
+// tiles per run of the CTA: the tiles take longer there, but no merge follows.  Measured
+// for one row (us, whole / equal runs and merge): d512 128 keys 11.1 / 17.3, 300 keys
+// 16.7 / 17.1, 400 keys 20.4 / 17.0; d256 300 keys 10.4 / 15.0, 700 keys 15.4 / 15.2,
+// 1100 keys 19.7 / 15.7; 32 columns d512 128 keys 13.8 / 16.3, 192 keys 17.1 / 15.4.
+constexpr int kWholeTiles = 2;
+
 // Launch shape and workspace of the attention.
 struct AttnPlan {
   int64_t tiles = 0;  // upper bound of the tile list
   int cols = 0, tile = 0, col_groups = 0;
   int ctas = 0;
+  bool whole = false;
   size_t part_o = 0, part_ml = 0, plan = 0, total = 0;
 };
 
@@ -134,6 +142,14 @@ AttnPlan attn_plan(const g4_kv8_args* a) {
   // one CTA per SM; fewer when there is less than a tile per run
   w.ctas = static_cast<int>(std::max<int64_t>(
       1, std::min<int64_t>(api_sm_count(), (w.tiles + shape.runs - 1) / shape.runs)));
+  // Few short items: a CTA each, which needs no parts and no merge.
+  const int64_t items = int64_t(a->batch) * a->num_kv_heads * w.col_groups;
+  w.whole = items <= api_sm_count() && per_item <= kWholeTiles * shape.runs;
+  if (w.whole) {
+    w.ctas = static_cast<int>(items);
+    w.total = 256;
+    return w;
+  }
   const size_t slots = size_t(w.ctas) * shape.runs * 2;
   size_t off = 0;
   w.plan = off;
@@ -322,6 +338,7 @@ int g4_kv8_attn(const g4_kv8_args* a, void* stream) {
   p.cols = w.cols;
   p.tile = w.tile;
   p.col_groups = w.col_groups;
+  p.whole = w.whole;
   p.q = static_cast<const __nv_bfloat16*>(a->q);
   p.o = static_cast<__nv_bfloat16*>(a->o);
   for (int i = 0; i < 3; ++i) {
@@ -342,7 +359,7 @@ int g4_kv8_attn(const g4_kv8_args* a, void* stream) {
     rc = launch_kv8_attn(a->head_dim, a->format == G4_KV8_INT8, p, w.ctas, st);
     if (rc) return launched(rc, "cache attention launch");
   }
-  if (w.ctas > 1) {  // one CTA sums its own parts
+  if (!w.whole && w.ctas > 1) {  // one CTA sums its own parts
     LaunchScope ls(kKKv8Merge, st);
     return launched(launch_kv8_merge(a->head_dim, p, w.ctas, st), "cache attention merge launch");
   }

@@ -97,6 +97,12 @@ struct TileList {
     }
     return pl;
   }
+  // The first tile of an item.
+  __device__ __forceinline__ Place item_place(int b, int item) const {
+    const RowPlan r = rows(b);
+    const bool act = item < active_items(r);
+    return {b, item, act ? r.lo / kTile : 0, act ? row_tiles(r, kTile) : 1};
+  }
   __device__ __forceinline__ void next_item(Place& pl) const {
     ++pl.item;
     if (pl.item >= p.cache.heads * p.col_groups) {
@@ -107,10 +113,7 @@ struct TileList {
         return;
       }
     }
-    const RowPlan r = rows(pl.b);
-    const bool act = pl.item < active_items(r);
-    pl.tile = act ? r.lo / kTile : 0;
-    pl.left = act ? row_tiles(r, kTile) : 1;
+    pl = item_place(pl.b, pl.item);
   }
   // KV head and column group of an item
   __device__ __forceinline__ void item_head(int b, int item, int& head, int& cg) const {

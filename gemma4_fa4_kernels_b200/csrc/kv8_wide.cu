@@ -183,18 +183,26 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv8_wide_kernel(const Kv8Attn
   const auto row_at = [&](int b) { return row_plan(p, b); };
   const TileList<kWideTile, N, decltype(row_at)> list{p, row_at, prefix};
   tc_fence_before();
-  plan_rows<kWideThreads>(p, list, prefix, misc->scan, [](int, const RowPlan&) {});
-  tc_fence_after();
-  const int total = prefix[p.rows.batch];
-  const int runs = min(total, static_cast<int>(gridDim.x));
-  if (blockIdx.x == 0 && tid == 0)
-    *reinterpret_cast<int4*>(p.plan) = make_int4(runs, total, 0, 0);
   const int W = blockIdx.x;
-  const int w_begin = W < runs ? run_begin(W, runs, total) : 0;
-  int todo = W < runs ? run_begin(W + 1, runs, total) - w_begin : 0;
+  Place pl;
+  int todo = 0;
+  if (p.whole) {
+    const int items = heads * p.col_groups, b = W / items;
+    __syncthreads();
+    pl = list.item_place(b, W - b * items);
+    todo = pl.left;
+  } else {
+    plan_rows<kWideThreads>(p, list, prefix, misc->scan, [](int, const RowPlan&) {});
+    const int total = prefix[p.rows.batch];
+    const int runs = min(total, static_cast<int>(gridDim.x));
+    if (W == 0 && tid == 0) *reinterpret_cast<int4*>(p.plan) = make_int4(runs, total, 0, 0);
+    const int begin = W < runs ? run_begin(W, runs, total) : 0;
+    if (W < runs) todo = run_begin(W + 1, runs, total) - begin;
+    pl = list.locate(begin);
+  }
+  tc_fence_after();
   const uint32_t tmem = misc->tmem_base;
   const CtaAbort ab{&misc->abort, nullptr};
-  Place pl = list.locate(w_begin);
   bool ok = true;
 
   if (warp > kSoft) {

@@ -44,7 +44,7 @@ import torch
 
 from . import _lib, ops
 from .errors import UnsupportedB200Path
-from .ops import _raise_for, _stream, _workspace
+from .ops import _raise_for, _stream
 
 PAGE_SIZES = (16, 32, 64, 128)
 CODE_DTYPES = {torch.float8_e4m3fn: _lib.G4_KV8_E4M3, torch.int8: _lib.G4_KV8_INT8}
@@ -57,6 +57,15 @@ MAX_ROWS = 1024
 #   d512, 17000 keys    256 columns 155 / 417, 386 / 587   512 columns  208 / 421, 724 / 589
 #   d256, window 1024    32 columns  30 / 37,   36 / 50     64 columns   42 / 36,   54 / 52
 DIRECT_COLUMNS = {512: 256, 256: 32}
+
+
+def _layout(*shape) -> tuple:
+    """(shape, strides) of a contiguous tensor."""
+    strides, n = [], 1
+    for x in reversed(shape):
+        strides.append(n)
+        n *= max(x, 1)
+    return shape, tuple(strides[::-1])
 
 
 def _strides(t: torch.Tensor) -> list[int]:
@@ -156,9 +165,15 @@ class PagedKVCache8:
             raise UnsupportedB200Path(f"at most {MAX_ROWS} rows per call")
 
     @staticmethod
-    def _no_grad(*tensors) -> None:
-        if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
-            raise UnsupportedB200Path("the paged cache is inference only: an operand requires grad")
+    def _grad(*tensors) -> None:
+        for t in tensors:
+            if t.requires_grad and torch.is_grad_enabled():
+                raise UnsupportedB200Path("the paged cache is inference only: an operand "
+                                          "requires grad")
+
+    # empty_strided takes half the host time of torch.empty
+    def _new(self, layout, dtype) -> torch.Tensor:
+        return torch.empty_strided(layout[0], layout[1], dtype=dtype, device=self.device)
 
     def _ints(self, t, rows: int | None, name: str) -> torch.Tensor:
         """``t``, a contiguous int32 vector of ``rows`` entries on the cache's device."""
@@ -228,8 +243,12 @@ class PagedKVCache8:
             a.second = second.data_ptr()
         ws = None
         if workspace:
-            ws = _workspace(_lib.load().g4_pages_workspace_bytes(ctypes.byref(a)), self.device)
-            a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
+            need = self._calls.get(("workspace", batch))
+            if need is None:
+                need = self._keep(("workspace", batch),
+                                  _lib.load().g4_pages_workspace_bytes(ctypes.byref(a)))
+            ws = torch.empty(need, dtype=torch.uint8, device=self.device)
+            a.workspace, a.workspace_bytes = ws.data_ptr(), need
         return a, ws
 
     # ----------------------------------------------------------------------------
@@ -242,7 +261,7 @@ class PagedKVCache8:
         key = ("append", layer, k.shape, k.stride(), k.dtype, k.device, v.shape, v.stride(),
                v.dtype, v.device)
         call = self._calls.get(key) or self._append_call(key, layer, k, v)
-        self._no_grad(k, v)
+        self._grad(k, v)
         batch, block = call
         if block is None:
             return
@@ -266,27 +285,28 @@ class PagedKVCache8:
         (rows, max_tokens, KV heads, head_dim), zeros past a row's end and where it
         has no page.  Exact for what :meth:`append` wrote."""
         batch = self._ints(starts, None, "starts").shape[0]
-        if batch > MAX_ROWS:
-            raise UnsupportedB200Path(f"at most {MAX_ROWS} rows per call")
-        if max_tokens < 0:
-            raise ValueError("max_tokens must be >= 0")
-        shape = (batch, max_tokens, self.num_kv_heads, self.head_dim)
-        k = torch.empty(shape, dtype=torch.bfloat16, device=self.device)
-        v = torch.empty_like(k)
+        key = ("read", layer, batch, max_tokens)
+        call = self._calls.get(key)
+        if call is None:
+            if batch > MAX_ROWS:
+                raise UnsupportedB200Path(f"at most {MAX_ROWS} rows per call")
+            if max_tokens < 0:
+                raise ValueError("max_tokens must be >= 0")
+            layout = _layout(batch, max_tokens, self.num_kv_heads, self.head_dim)
+            call = self._keep(key, (layout, self._read_block(layer, batch, max_tokens)))
+        layout, block = call
+        k, v = self._new(layout, torch.bfloat16), self._new(layout, torch.bfloat16)
         if batch and max_tokens:
-            self._read(layer, slots, starts, ends, k, v, batch, max_tokens, None)
-        elif not 0 <= layer < self.num_layers:
-            raise IndexError(f"layer {layer} of a cache of {self.num_layers}")
+            self._read(block, batch, slots, starts, ends, k, v, None)
         return k, v
 
-    def _read(self, layer, slots, starts, ends, k, v, batch, tokens, out_rows) -> None:
-        key = ("read", layer, batch, tokens, out_rows is None)
-        block = self._calls.get(key)
-        if block is None:
-            a = self._block(layer, batch, tokens)
-            row = self.num_kv_heads * self.head_dim
-            a.k_stride[:] = a.v_stride[:] = (tokens * row, row, self.head_dim)
-            block = self._keep(key, bytes(a))
+    def _read_block(self, layer, batch, tokens) -> bytes:
+        a = self._block(layer, batch, tokens)
+        row = self.num_kv_heads * self.head_dim
+        a.k_stride[:] = a.v_stride[:] = (tokens * row, row, self.head_dim)
+        return bytes(a)
+
+    def _read(self, block, batch, slots, starts, ends, k, v, out_rows) -> None:
         a = _lib.G4Kv8Args.from_buffer_copy(block)
         self._rows(a, batch, slots, starts, ends)
         a.k, a.v = k.data_ptr(), v.data_ptr()
@@ -310,18 +330,17 @@ class PagedKVCache8:
         """
         key = ("attention", layer, window, max_seqlen_k, q.shape, q.stride(), q.dtype, q.device)
         call = self._calls.get(key) or self._attention_call(key, layer, q, window, max_seqlen_k)
-        self._no_grad(q)
-        batch, block, lse_shape, ws_bytes, chunk = call
+        self._grad(q)
+        batch, block, out_layout, lse_layout, ws_bytes, chunk = call
+        out = self._new(out_layout, torch.bfloat16)
         if block is None:
-            return (torch.empty(q.shape, dtype=torch.bfloat16, device=self.device),
-                    torch.empty(lse_shape, dtype=torch.float32, device=self.device))
+            return out, self._new(lse_layout, torch.float32)
         a = _lib.G4Kv8Args.from_buffer_copy(block)
         self._rows(a, batch, slots, starts, ends)
-        out = torch.empty(q.shape, dtype=torch.bfloat16, device=self.device)
         a.o = out.data_ptr()
         if chunk:
             return out, self._chunk(a, layer, q, out, slots)
-        lse = torch.empty(lse_shape, dtype=torch.float32, device=self.device)
+        lse = self._new(lse_layout, torch.float32)
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=self.device)
         a.q, a.lse, a.workspace = q.data_ptr(), lse.data_ptr(), ws.data_ptr()
         self._launch(_lib.load().g4_kv8_attn, ctypes.byref(a))
@@ -343,8 +362,9 @@ class PagedKVCache8:
         a.o_stride[:] = (heads * tokens * d, heads * d, d)
         if any(s <= 0 or s % 8 for s in a.q_stride):
             raise ValueError("q strides must be positive multiples of 8 elements")
+        layouts = _layout(batch, tokens, heads, d), _layout(batch, heads, tokens)
         if not batch or not tokens:
-            return self._keep(key, (batch, None, (batch, heads, tokens), 0, False))
+            return self._keep(key, (batch, None, *layouts, 0, False))
         chunk = tokens * (heads // self.num_kv_heads) > DIRECT_COLUMNS[d]
         if chunk:  # LSE as the packed forward writes it: (head, row, token)
             a.lse_stride[:] = (tokens, batch * tokens)
@@ -354,7 +374,7 @@ class PagedKVCache8:
             a.starts = a.ends = 16  # the size does not depend on the call's pointers
             ws_bytes = _lib.load().g4_kv8_attn_workspace_bytes(ctypes.byref(a))
             a.workspace_bytes = ws_bytes
-        return self._keep(key, (batch, bytes(a), (batch, heads, tokens), ws_bytes, chunk))
+        return self._keep(key, (batch, bytes(a), *layouts, ws_bytes, chunk))
 
     def _chunk(self, a, layer, q, out, slots):
         batch, tokens, heads, d = q.shape
@@ -372,7 +392,7 @@ class PagedKVCache8:
         k = torch.empty((batch * keys, self.num_kv_heads, d), dtype=torch.bfloat16,
                         device=self.device)
         v = torch.empty_like(k)
-        self._read(layer, slots, first, last, k, v, batch, keys, cu_k)
+        self._read(self._read_block(layer, batch, keys), batch, slots, first, last, k, v, cu_k)
         with torch.cuda.device(self.device):
             _, lse = ops.attn_fwd(q.reshape(total, heads, d), k, v, window=window,
                                   cu_seqlens_q=cu_q, cu_seqlens_k=cu_k, max_seqlen_q=tokens,
@@ -393,7 +413,8 @@ class PagedKVCache8:
         if isinstance(counts, int):
             counts = torch.full((batch,), counts, dtype=torch.int32, device=self.device)
         self._ints(counts, batch, "counts")
-        starts, ends = torch.empty((2, batch), dtype=torch.int32, device=self.device).unbind(0)
+        starts = torch.empty(batch, dtype=torch.int32, device=self.device)
+        ends = torch.empty_like(starts)
         if batch:
             a, _ = self._pages(batch, slots)
             a.counts, a.starts, a.ends = counts.data_ptr(), starts.data_ptr(), ends.data_ptr()
