@@ -12,7 +12,7 @@
 // swizzle), which the MMA reads once: 4 bytes of shared-memory traffic per code, at
 // 128 bytes per clock 32 codes per clock and SM, against the SM's share of HBM of 23;
 // in practice the converters' issue slots and the waits between tiles.  Five drafted
-// tokens of 8 heads (40 columns) over 6 rows of 700 to 9001 int8 keys: 57 us with 14 us for
+// tokens of 8 heads (40 columns) over 6 rows of 700 to 9001 int8 keys: 53 us with 14 us for
 // the merge behind it, 94 and 12 with three blocks of 8 columns per pass of mma.sync.
 //
 // Warp roles: 8 softmax warps (two per 32 TMEM lanes, thread = key, half of the columns
@@ -221,9 +221,10 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv8_wide_kernel(const Kv8Attn
     RowPlan row;
     int f_hi = 0;
     // pool row (page, head, token) of the thread's rows r0 + 16 j in the next chunk's
-    // operand, -1: a zero row; its table entries are requested a chunk earlier
+    // operand; its table entries are requested a chunk earlier.  Rows that no column sees
+    // are zeros, whatever the pool holds: they load row 0, and `live` leaves them out.
     int from[8], entry[8];
-    bool f_all = false;   // no zero rows in the tile
+    uint32_t live = 0, live_next = 0;   // bit j: row r0 + 16 j
     auto next_operand = [&]() {
       if (f_v == f_n) {  // the next item
         if (f_n > 0) {
@@ -262,23 +263,19 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv8_wide_kernel(const Kv8Attn
     };
     auto next_chunk = [&]() {  // from the entries to rows
       pool = pool_next;
-      bool all = true;
+      live_next = 0;
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const int key = d_tile * kWideTile + r0 + 16 * j;
         const bool ok_page = entry[j] >= 0 && entry[j] < p.cache.num_pages;
         from[j] = ok_page ? (entry[j] * heads + d_head) * p.cache.page + (key & (p.cache.page - 1))
-                          : -1;
-        all = all && ok_page;
+                          : 0;
+        live_next |= ok_page ? 1u << j : 0u;
       }
-      f_all = __all_sync(0xffffffffu, all);
     };
     auto fetch = [&](int j) {  // row block j / 2, half j % 2
-      const uint4* src = reinterpret_cast<const uint4*>(
-          pool + static_cast<int64_t>(from[j >> 1]) * D + (j & 1) * 64);
-      if (f_all) return __ldcs(src);
-      // rows that no column sees are zeros, whatever the page holds there
-      return from[j >> 1] >= 0 ? __ldcs(src) : make_uint4(0u, 0u, 0u, 0u);
+      return __ldcs(reinterpret_cast<const uint4*>(
+          pool + static_cast<int64_t>(from[j >> 1]) * D + (j & 1) * 64));
     };
     const int chunks = todo * 2 * kChunks;  // of the run; this pair's are feed, feed + 3, ...
     uint32_t stage = feed % kStages, phase = 0;
@@ -291,8 +288,13 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv8_wide_kernel(const Kv8Attn
     }
 #pragma unroll 1
     for (int q = feed; q < chunks && ok; q += kFeeds) {
-      const bool more = q + kFeeds < chunks;
-      if (more) next_chunk();
+      live = live_next;
+      if (q + kFeeds < chunks) next_chunk();  // else the last chunk's rows once more, unused
+      if (__any_sync(0xffffffffu, live != 255u)) {
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+          if (!(live >> (j >> 1) & 1u)) raw[j] = make_uint4(0u, 0u, 0u, 0u);
+      }
       if (q + 2 * kFeeds < chunks) look_ahead();
       ok = mbar_wait(&misc->empty[stage], phase ^ 1, ab, kDevTimeoutMma);
       uint8_t* st = ring + stage * kStageBytes;
@@ -307,7 +309,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv8_wide_kernel(const Kv8Attn
         uint8_t* dst = st + (j >> 1) * 2048 + (j & 1) * 16384;
         *reinterpret_cast<uint4*>(dst + at0) = make_uint4(h[0], h[1], h[2], h[3]);
         *reinterpret_cast<uint4*>(dst + at1) = make_uint4(h[4], h[5], h[6], h[7]);
-        if (more) raw[j] = fetch(j);  // the pair's next chunk, a chunk's time ahead
+        raw[j] = fetch(j);  // the pair's next chunk, a chunk's time ahead
       }
       fence_proxy_async_smem();
       __syncwarp();
