@@ -132,7 +132,7 @@ struct Kv8AttnParams {
   float* part_o;            // [slot][cols][head_dim]
   float4* part_ml;          // [slot][cols]: (shift of O, max, sum, -)
   int* status;              // nullable
-  int* plan;                // (not used if whole) {runs, tiles, -, -}, the rows' plans (int4 each), their first tiles
+  int* plan;                // (not used if whole) {runs, entries, kOver, -}, the rows' plans (int4 each), their first tiles
 };
 // The kernel's launch shape for a row's number of (token, query head) columns.
 struct Kv8AttnShape {

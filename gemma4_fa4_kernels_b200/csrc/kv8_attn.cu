@@ -52,6 +52,8 @@ namespace g4 {
 
 namespace {
 
+constexpr int kOver = 1;  // entries of the tile list that stand for taking up an item
+
 // A launch shape: kTeam warps share a run; one pass over the codes serves 8 columns.
 template <int kD, int kTeam_, int kWarps_, int kBufs_>
 struct AttnShape {
@@ -127,9 +129,9 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1) kv8_attn_kernel(const Kv8Att
   pdl_enter();
   const int B = p.rows.batch, heads = p.cache.heads;
   const auto row_at = [&](int b) { return rows[b]; };
-  const TileList<kKv8Tile, kCols, decltype(row_at)> list{p, row_at, prefix};
+  const TileList<kKv8Tile, kCols, kOver, decltype(row_at)> list{p, row_at, prefix};
   const int W = blockIdx.x * Cfg::kTeams + team;
-  Place first;
+  Place first = {0, 0, 0, 0};
   int todo = 0;
   if (p.whole) {  // the CTA's item, cut into a run per team
     const int items = heads * p.col_groups, b = blockIdx.x / items;
@@ -148,10 +150,13 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1) kv8_attn_kernel(const Kv8Att
     const int total = prefix[B];
     const int runs = min(total, static_cast<int>(gridDim.x) * Cfg::kTeams);
     if (blockIdx.x == 0 && tid == 0)
-      *reinterpret_cast<int4*>(p.plan) = make_int4(runs, total, 0, 0);
-    const int begin = W < runs ? run_begin(W, runs, total) : 0;
-    if (W < runs) todo = run_begin(W + 1, runs, total) - begin;
-    first = list.locate(begin);
+      *reinterpret_cast<int4*>(p.plan) = make_int4(runs, total, kOver, 0);
+    if (W < runs) {
+      int t0, t1;
+      list.locate(run_begin(W + 1, runs, total), t1);
+      first = list.locate(run_begin(W, runs, total), t0);
+      todo = t1 - t0;
+    }
   }
 
   // ---- the loading side: 16-key pieces in order K0a K0b V0a V0b K1a ... ----
@@ -237,8 +242,6 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1) kv8_attn_kernel(const Kv8Att
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
-#pragma unroll 1
-  for (int i = 0; i < Cfg::kBufs; ++i) request();
 
   // ---- the computing side ----
   uint32_t qf[Cfg::kChunks][8];
@@ -365,9 +368,16 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1) kv8_attn_kernel(const Kv8Att
     }
   };
 
-  bool open = false;           // an item is in progress
+  bool open = todo > 0;        // an item is in progress
   bool from_start = false;     // its first tile lies in this run
-  if (todo > 0) from_start = list.at_start(pl);
+  if (open) {
+    // the first queries before the first codes: behind a whole ring's requests of every
+    // warp they would come 2 to 3 us later
+    from_start = list.at_start(pl);
+    begin_item();
+  }
+#pragma unroll 1
+  for (int i = 0; i < Cfg::kBufs; ++i) request();
 #pragma unroll 1
   while (todo > 0) {
     if (!open) {
@@ -657,15 +667,15 @@ __global__ void __launch_bounds__(kThreads) kv8_merge_kernel(const Kv8AttnParams
   const int4 head4 = *reinterpret_cast<const int4*>(p.plan);
   const int4 row4 = reinterpret_cast<const int4*>(p.plan)[1 + b];
   const int row_first = p.plan[4 + 4 * B + b];
-  const int runs = head4.x, total = head4.y;
+  const int runs = head4.x, total = head4.y, over = head4.z;
   const RowPlan r = {row4.x, row4.y, row4.z, row4.w};
   const int act = (r.n * p.group + p.cols - 1) / p.cols;
   if (grp >= act) return;  // padding: written by the run that met it
   const int nt = row_tiles(r, p.tile);
-  const int i0 = row_first + (h * act + grp) * nt, i1 = i0 + nt;
+  const int i0 = row_first + (h * act + grp) * (nt + over), i1 = i0 + nt;
   const int w0 = run_of(i0, runs, total), w1 = run_of(i1 - 1, runs, total);
-  if (w0 == w1) return;                                       // one run had it all
-  const bool has_head = i1 < run_begin(w1 + 1, runs, total);  // ends inside run w1
+  if (w0 == w1) return;                                           // one run had it all
+  const bool has_head = i1 + over < run_begin(w1 + 1, runs, total);  // run w1 goes on behind it
   if (!has_head && w0 / teams == w1 / teams) return;          // one CTA had it all
   // CTAs that hold a tail of it
   const int c0 = w0 / teams, c1 = (has_head ? w1 - 1 : w1) / teams;

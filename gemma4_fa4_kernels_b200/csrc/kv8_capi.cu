@@ -138,7 +138,8 @@ AttnPlan attn_plan(const g4_kv8_args* a) {
   int64_t keys = a->max_seqlen_k;
   if (a->window > 0) keys = std::min<int64_t>(keys, int64_t(a->window) + a->tokens - 1);
   const int64_t per_item = (keys + shape.tile - 1) / shape.tile + 1;
-  w.tiles = int64_t(a->batch) * a->num_kv_heads * w.col_groups * per_item;
+  // (with what the list counts for taking up an item)
+  w.tiles = int64_t(a->batch) * a->num_kv_heads * w.col_groups * (per_item + 2);
   // one CTA per SM; fewer when there is less than a tile per run
   w.ctas = static_cast<int>(std::max<int64_t>(
       1, std::min<int64_t>(api_sm_count(), (w.tiles + shape.runs - 1) / shape.runs)));

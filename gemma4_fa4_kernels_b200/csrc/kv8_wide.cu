@@ -12,7 +12,7 @@
 // swizzle), which the MMA reads once: 4 bytes of shared-memory traffic per code, at
 // 128 bytes per clock 32 codes per clock and SM, against the SM's share of HBM of 23;
 // in practice the converters' issue slots and the waits between tiles.  Five drafted
-// tokens of 8 heads (40 columns) over 6 rows of 700 to 9001 int8 keys: 53 us with 14 us for
+// tokens of 8 heads (40 columns) over 6 rows of 700 to 9001 int8 keys: 45 us with 14 us for
 // the merge behind it, 94 and 12 with three blocks of 8 columns per pass of mma.sync.
 //
 // Warp roles: 8 softmax warps (two per 32 TMEM lanes, thread = key, half of the columns
@@ -35,6 +35,7 @@ namespace g4 {
 namespace {
 
 constexpr int kWideTile = 128;
+constexpr int kWideOver = 2;       // entries of the tile list that stand for taking up an item
 constexpr int kStageBytes = 32768;
 constexpr int kSoft = 8;           // softmax warps
 constexpr int kFeeds = 3;          // pairs of converter warps
@@ -181,10 +182,10 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv8_wide_kernel(const Kv8Attn
   pdl_enter();
   const int heads = p.cache.heads;
   const auto row_at = [&](int b) { return row_plan(p, b); };
-  const TileList<kWideTile, N, decltype(row_at)> list{p, row_at, prefix};
+  const TileList<kWideTile, N, kWideOver, decltype(row_at)> list{p, row_at, prefix};
   tc_fence_before();
   const int W = blockIdx.x;
-  Place pl;
+  Place pl = {0, 0, 0, 0};
   int todo = 0;
   if (p.whole) {
     const int items = heads * p.col_groups, b = W / items;
@@ -195,10 +196,13 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv8_wide_kernel(const Kv8Attn
     plan_rows<kWideThreads>(p, list, prefix, misc->scan, [](int, const RowPlan&) {});
     const int total = prefix[p.rows.batch];
     const int runs = min(total, static_cast<int>(gridDim.x));
-    if (W == 0 && tid == 0) *reinterpret_cast<int4*>(p.plan) = make_int4(runs, total, 0, 0);
-    const int begin = W < runs ? run_begin(W, runs, total) : 0;
-    if (W < runs) todo = run_begin(W + 1, runs, total) - begin;
-    pl = list.locate(begin);
+    if (W == 0 && tid == 0) *reinterpret_cast<int4*>(p.plan) = make_int4(runs, total, kWideOver, 0);
+    if (W < runs) {
+      int t0, t1;
+      list.locate(run_begin(W + 1, runs, total), t1);
+      pl = list.locate(run_begin(W, runs, total), t0);
+      todo = t1 - t0;
+    }
   }
   tc_fence_after();
   const uint32_t tmem = misc->tmem_base;
