@@ -762,8 +762,10 @@ int launch_kv8_merge(int d, const Kv8AttnParams& p, int ctas, cudaStream_t strea
   const int items = p.rows.batch * p.cache.heads * p.col_groups;
   const int columns = std::min(p.cols, p.rows.tokens * p.group);
   const int units = columns * (d / 4);
-  // parts per item: about one per CTA that it spans
-  if (ctas >= 8 * items)
+  // Parts per item: about one per CTA that it spans.  Eight threads per unit pay off as
+  // long as they make no more CTAs than the GPU holds at once (16 items of 64
+  // columns: a call of 71 us with their 4096 CTAs, of 38 us with one thread per unit).
+  if (ctas >= 8 * items && int64_t(items) * units <= 128 * ctas)
     return static_cast<int>(launch_chained(kv8_merge_kernel<8, 256, 8>,
                                            dim3(items, (units + 31) / 32), dim3(256), 0, stream, p,
                                            d, teams));

@@ -53,10 +53,10 @@ MAX_ROWS = 1024
 # Up to this many (token, query head) columns per KV head and row, by head dim, the
 # queries read the codes directly; longer chunks of prompts run the tensor-core forward
 # over a BF16 copy of the keys they see.  Measured, us, direct against copy (1 and 4 rows):
-#   d512, 1500 keys     256 columns  69 / 63,   73 / 81    512 columns   52 / 65,  120 / 83
-#   d512, 17000 keys    256 columns 155 / 417, 386 / 587   512 columns  208 / 421, 724 / 589
-#   d256, window 1024    32 columns  30 / 37,   36 / 50     64 columns   42 / 36,   54 / 52
-DIRECT_COLUMNS = {512: 256, 256: 32}
+#   d512, 1500 keys     256 columns  38 / 65,   71 / 81    512 columns   46 / 67,  116 / 85
+#   d512, 17000 keys    256 columns 118 / 419, 374 / 587   512 columns  206 / 423, 712 / 595
+#   d256, window 1024    64 columns  32 / 36,   48 / 52    128 columns   34 / 36,   75 / 52
+DIRECT_COLUMNS = {512: 256, 256: 64}
 
 
 def _layout(*shape) -> tuple:
