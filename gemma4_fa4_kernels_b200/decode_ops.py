@@ -28,8 +28,8 @@ Q/K norms, the rotary embedding and the value norm run in the fused
 the same layers over a :class:`~gemma4_fa4_kernels_b200.PagedKVCache8`: a batch of
 sequences of any lengths, one or several (drafted) tokens or a chunk of a prompt
 each, the new K and V appended as 8-bit codes.  Lengths and tables stay on the
-device, so these calls never wait for it and can be captured into a graph; the
-cache is an object, so they are plain functions and not custom ops.
+device, so these calls do not wait for it and decode steps can be captured into a
+graph; the cache is an object, so they are plain functions and not custom ops.
 """
 
 from __future__ import annotations

@@ -33,7 +33,10 @@ Slots of one call must be distinct.
 Head dims 256 and 512 (local and global layers), any number of query heads per KV
 head, softmax scale 1, the causal and sliding-window masks of the attention
 operators without vision or document ids.  Inference only.  Calls run on the
-current stream of the cache's device and never synchronise it (but ``check``).
+current stream of the cache's device and do not wait for it, except ``check`` and,
+for prompt chunks whose scratch exceeds the forward's budget, ``attention`` (as the
+packed forward does; such a call cannot be captured).  The cache's tensors are its own
+for its life: their contents may be changed from outside, they are not to be replaced.
 """
 
 from __future__ import annotations
@@ -179,7 +182,7 @@ class PagedKVCache8:
         """``t``, a contiguous int32 vector of ``rows`` entries on the cache's device."""
         if (isinstance(t, torch.Tensor) and t.dtype is torch.int32 and t.dim() == 1
                 and t.device == self.device and t.is_contiguous()
-                and (rows is None or t.shape[0] == rows)):
+                and (rows is None or len(t) == rows)):
             return t
         if not isinstance(t, torch.Tensor) or t.dtype != torch.int32 or t.dim() != 1:
             raise ValueError(f"{name} must be a one-dimensional int32 tensor")
