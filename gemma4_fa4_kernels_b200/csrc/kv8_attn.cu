@@ -242,6 +242,8 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1) kv8_attn_kernel(const Kv8Att
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
+#pragma unroll 1
+  for (int i = 0; i < Cfg::kBufs; ++i) request();
 
   // ---- the computing side ----
   uint32_t qf[Cfg::kChunks][8];
@@ -368,16 +370,9 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1) kv8_attn_kernel(const Kv8Att
     }
   };
 
-  bool open = todo > 0;        // an item is in progress
+  bool open = false;           // an item is in progress
   bool from_start = false;     // its first tile lies in this run
-  if (open) {
-    // the first queries before the first codes: behind a whole ring's requests of every
-    // warp they would come 2 to 3 us later
-    from_start = list.at_start(pl);
-    begin_item();
-  }
-#pragma unroll 1
-  for (int i = 0; i < Cfg::kBufs; ++i) request();
+  if (todo > 0) from_start = list.at_start(pl);
 #pragma unroll 1
   while (todo > 0) {
     if (!open) {
