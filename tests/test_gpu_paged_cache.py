@@ -381,6 +381,72 @@ def test_wide_maxima_that_rise_and_scales_of_any_size(fmt, d, group, tokens):
     check_attention(p, 0, q, [0], [n - tokens], [n])
 
 
+@pytest.mark.parametrize("seed", range(8))
+def test_random_batches_over_the_tile_list(seed):
+    """Rows of any length (none among them) in any order, bad slots, missing pages, padded
+    tokens, windows: in slots long enough that items share CTAs and span them."""
+    rng = np.random.default_rng(500 + seed)
+    d, heads, group = ((512, 1, 8), (256, 2, 2), (512, 2, 4), (256, 3, 1))[seed % 4]
+    tokens = (1, 1, 2, 7)[(seed + seed // 4) % 4]
+    page = int(rng.choice([16, 32, 64, 128]))
+    window = int(rng.choice([0, 100]))
+    n = int(rng.integers(3, 40))
+    lens = [int(x) for x in np.exp(rng.uniform(0, np.log(700), n))]
+    p = Pair("e4m3" if seed % 2 else "int8", heads=heads, page=page, d=d, slots=n,
+             pages=2 + sum(-(-x // page) for x in lens), per_slot=2048 // page)
+    p.fill(list(range(n)), lens, rng)
+    for slot in rng.choice(n, 2, replace=False):  # holes
+        p.ref.tables[slot, rng.integers(0, -(-lens[slot] // page))] = -1
+    p.dev.tables.copy_(i32(p.ref.tables))
+    rows = [int(x) for x in rng.permutation(n)]
+    ends = [lens[r] for r in rows]
+    new = [min(int(rng.integers(0, tokens + 1)), e) for e in ends]
+    rows[1] = n + 3
+    q = 0.3 * rng.standard_normal((n, tokens, heads * group, d))
+    check_attention(p, 0, q, rows, [e - m for e, m in zip(ends, new)], ends, window=window)
+
+
+def test_empty_rows_and_holes_in_long_slots():
+    rng = np.random.default_rng(23)
+    p = Pair("int8", heads=2, d=256, page=16, pages=80, slots=8, per_slot=64)
+    lens = [100, 37, 900, 20, 1]
+    p.fill([0, 1, 2, 3, 4], lens, rng)
+    p.ref.tables[1, :] = -1
+    p.ref.tables[2, 3:20] = -1
+    p.dev.tables.copy_(i32(p.ref.tables))
+    q = 0.3 * rng.standard_normal((9, 2, 4, 256))
+    args = ([0, 1, 2, 3, 4, 5, 9, -2, 0], [98, 35, 898, 18, 0, 0, 3, 3, 1022],
+            [100, 37, 900, 20, 1, 0, 5, 5, 1025])
+    check_attention(p, 0, q, *args)
+    check_attention(p, 0, q, *args, window=64)
+    got = check_attention(p, 0, q, *args, max_seqlen_k=899)
+    assert not got[2].any() and got[0].any()
+
+
+def test_calls_of_one_cache_on_two_streams():
+    """Reads of one cache need no order among themselves."""
+    rng = np.random.default_rng(24)
+    p = Pair("e4m3", heads=2, d=512, page=32, pages=140, slots=4, per_slot=80)
+    lens = [2000, 31, 1500, 400]
+    p.fill([0, 1, 2, 3], lens, rng)
+    slots, ends = i32([0, 1, 2, 3]), i32(lens)
+    ops = []
+    for tokens in (1, 4, 9):  # decode, wide of 32 and of 64 columns (group 4 and 8)
+        q, _ = bf16(0.3 * rng.standard_normal((4, tokens, 16, 512)))
+        ops.append((q, i32([x - tokens for x in lens])))
+    want = [p.dev.attention(0, q, slots, s, ends) for q, s in ops]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = []
+    for rep in range(4):
+        for i, (q, s) in enumerate(ops):
+            with torch.cuda.stream(streams[(i + rep) % 2]):
+                got.append((i, p.dev.attention(0, q, slots, s, ends)))
+    torch.cuda.synchronize()
+    for i, (out, lse) in got:
+        assert torch.equal(out, want[i][0]) and torch.equal(lse, want[i][1])
+
+
 def test_wide_empty_rows_masked_pages_and_stale_slots():
     rng = np.random.default_rng(21)
     p = Pair("e4m3", heads=1, d=512, page=16, pages=40, slots=8, per_slot=20)
