@@ -104,6 +104,8 @@ Kv8Rows rows_of(const g4_kv8_args* a) {
 int check_attn_shape(const g4_kv8_args* a) {
   if (a->num_q_heads <= 0 || a->num_q_heads % a->num_kv_heads)
     return api_fail(G4_ERR_INVALID, "query heads must be a positive multiple of KV heads");
+  if (int64_t(a->num_q_heads / a->num_kv_heads) * a->tokens > (1 << 30))
+    return api_fail(G4_ERR_UNSUPPORTED, "too many (token, query head) columns per KV head");
   if (a->window < 0) return api_fail(G4_ERR_INVALID, "window must be >= 0");
   if (a->max_seqlen_k <= 0 ||
       a->max_seqlen_k > static_cast<int64_t>(a->pages_per_slot) * a->page_size)
@@ -138,13 +140,15 @@ AttnPlan attn_plan(const g4_kv8_args* a) {
   int64_t keys = a->max_seqlen_k;
   if (a->window > 0) keys = std::min<int64_t>(keys, int64_t(a->window) + a->tokens - 1);
   const int64_t per_item = (keys + shape.tile - 1) / shape.tile + 1;
+  // capped, so that the product below fits; the call is refused long before
+  const int64_t items =
+      std::min<int64_t>(int64_t(a->batch) * a->num_kv_heads * w.col_groups, int64_t(1) << 32);
   // (with what the list counts for taking up an item)
-  w.tiles = int64_t(a->batch) * a->num_kv_heads * w.col_groups * (per_item + 2);
+  w.tiles = items * (per_item + 2);
   // one CTA per SM; fewer when there is less than a tile per run
   w.ctas = static_cast<int>(std::max<int64_t>(
       1, std::min<int64_t>(api_sm_count(), (w.tiles + shape.runs - 1) / shape.runs)));
   // Few short items: a CTA each, which needs no parts and no merge.
-  const int64_t items = int64_t(a->batch) * a->num_kv_heads * w.col_groups;
   w.whole = items <= api_sm_count() && per_item <= kWholeTiles * shape.runs;
   if (w.whole) {
     w.ctas = static_cast<int>(items);

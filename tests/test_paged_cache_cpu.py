@@ -163,6 +163,13 @@ def _kv8(**over):
     ("g4_kv8_attn", dict(), _lib.G4_ERR_WORKSPACE, "workspace"),
     ("g4_kv8_attn", dict(batch=1024, tokens=1 << 20, workspace=0x10000, workspace_bytes=1 << 40),
      _lib.G4_ERR_UNSUPPORTED, "tiles"),
+    # a product of sizes past 64 bits
+    ("g4_kv8_attn", dict(batch=1024, tokens=1 << 24, num_q_heads=65535 * 64, num_kv_heads=65535,
+                         page_size=16, num_pages=1, pages_per_slot=1 << 26,
+                         max_seqlen_k=((1 << 13) - 2) * 128, workspace=0x10000,
+                         workspace_bytes=1 << 40), _lib.G4_ERR_UNSUPPORTED, "tiles"),
+    ("g4_kv8_attn", dict(batch=1, tokens=1 << 24, num_q_heads=512), _lib.G4_ERR_UNSUPPORTED,
+     "columns"),
     ("g4_kv8_pad_rows", dict(o=None), _lib.G4_ERR_INVALID, "o is required"),
 ])
 def test_cache_calls_fail_before_launch(fn, over, code, needle):
