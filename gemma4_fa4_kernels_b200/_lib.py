@@ -13,7 +13,7 @@ import threading
 _PKG_DIR = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_PKG_DIR, "libgemma4_b200.so")
 
-ABI_VERSION = 2
+ABI_VERSION = 3
 
 G4_OK = 0
 G4_ERR_INVALID = 1
@@ -199,6 +199,7 @@ class G4Kv8Args(ctypes.Structure):
         ("v_stride", ctypes.c_int64 * 3),
         ("out_rows", ctypes.c_void_p),
         ("out_total", ctypes.c_int32),
+        ("holes", ctypes.c_void_p),
         ("q", ctypes.c_void_p),
         ("o", ctypes.c_void_p),
         ("lse", ctypes.c_void_p),

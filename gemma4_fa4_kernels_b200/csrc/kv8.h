@@ -122,6 +122,9 @@ struct Kv8AttnParams {
   int tile;                 // keys per tile of the list
   int col_groups;           // ceil(tokens * group / cols)
   bool whole;               // one CTA per item instead of equal runs: nothing to merge
+  const int* only;          // nullable: the rows whose flag is set, `per_row` CTAs each; the
+                            // other rows' padding is cleared
+  int per_row;
   const __nv_bfloat16* q;   // (batch, token, head) strides in elements
   int64_t q_stride[3];
   __nv_bfloat16* o;
@@ -160,6 +163,7 @@ struct Kv8StoreParams {
   int64_t out_stride[3];
   const int* out_rows;      // read, nullable: rows packed, row b at [out_rows[b], out_rows[b+1])
   int out_total;            // packed: rows of the output
+  int* holes;               // read, nullable: [b] = 1 where a position of row b has no page
   int* status;              // nullable
 };
 int launch_kv8_append(int d, bool int8, const Kv8StoreParams& p, cudaStream_t stream);
@@ -174,12 +178,9 @@ struct Kv8ChunkParams {
   int* cu_k;                // [batch + 1]
   int* first;               // [batch] first key read
   int* last;                // [batch] one past the last key read
+  int* holes;               // [batch] cleared
 };
 int launch_kv8_chunk_plan(const Kv8ChunkParams& p, cudaStream_t stream);
-// zeros (LSE: -inf) in the rows of a chunk's output that are padding
-int launch_kv8_pad_rows(const Kv8Cache& c, const Kv8Rows& r, int max_k, int heads, int d,
-                        __nv_bfloat16* o, const int64_t* o_stride, float* lse,
-                        const int64_t* lse_stride, cudaStream_t stream);
 
 // ---- pages (kv8_pages.cu) ----
 struct Kv8PagesParams {

@@ -167,6 +167,28 @@ AttnPlan attn_plan(const g4_kv8_args* a) {
   return w;
 }
 
+// Operands of an attention launch; its shape is still to be set.
+Kv8AttnParams attn_of(const g4_kv8_args* a) {
+  Kv8AttnParams p;
+  memset(&p, 0, sizeof(p));
+  p.cache = cache_of(a);
+  p.rows = rows_of(a);
+  p.window = a->window;
+  p.max_k = a->max_seqlen_k;
+  p.group = a->num_q_heads / a->num_kv_heads;
+  p.q = static_cast<const __nv_bfloat16*>(a->q);
+  p.o = static_cast<__nv_bfloat16*>(a->o);
+  for (int i = 0; i < 3; ++i) {
+    p.q_stride[i] = a->q_stride[i];
+    p.o_stride[i] = a->o_stride[i];
+  }
+  p.lse = a->lse;
+  p.lse_stride[0] = a->lse_stride[0];
+  p.lse_stride[1] = a->lse_stride[1];
+  p.status = a->status;
+  return p;
+}
+
 int check_pages(const g4_pages_args* a) {
   if (!a) return api_fail(G4_ERR_INVALID, "null argument block");
   if (!a->tables || !a->lengths || !a->refcounts || !a->status)
@@ -300,6 +322,7 @@ int g4_kv8_read(const g4_kv8_args* a, void* stream) {
   for (int i = 0; i < 3; ++i) p.out_stride[i] = a->k_stride[i];
   p.out_rows = a->out_rows;
   p.out_total = a->out_total;
+  p.holes = a->holes;
   const OnDevice guard(a->device);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   LaunchScope ls(kKKv8Read, st);
@@ -333,28 +356,12 @@ int g4_kv8_attn(const g4_kv8_args* a, void* stream) {
   if (!a->workspace || !al16(a->workspace) || a->workspace_bytes < w.total)
     return api_fail(G4_ERR_WORKSPACE, "a 16-byte aligned workspace of %zu bytes is required",
                     w.total);
-  Kv8AttnParams p;
-  memset(&p, 0, sizeof(p));
-  p.cache = cache_of(a);
-  p.rows = rows_of(a);
-  p.window = a->window;
-  p.max_k = a->max_seqlen_k;
-  p.group = a->num_q_heads / a->num_kv_heads;
+  Kv8AttnParams p = attn_of(a);
   p.cols = w.cols;
   p.tile = w.tile;
   p.col_groups = w.col_groups;
   p.whole = w.whole;
-  p.q = static_cast<const __nv_bfloat16*>(a->q);
-  p.o = static_cast<__nv_bfloat16*>(a->o);
-  for (int i = 0; i < 3; ++i) {
-    p.q_stride[i] = a->q_stride[i];
-    p.o_stride[i] = a->o_stride[i];
-  }
-  p.lse = a->lse;
-  p.lse_stride[0] = a->lse_stride[0];
-  p.lse_stride[1] = a->lse_stride[1];
   uint8_t* ws = static_cast<uint8_t*>(a->workspace);
-  p.status = a->status;
   p.plan = reinterpret_cast<int*>(ws + w.plan);
   p.part_ml = reinterpret_cast<float4*>(ws + w.part_ml);
   p.part_o = reinterpret_cast<float*>(ws + w.part_o);
@@ -383,6 +390,7 @@ int g4_kv8_chunk_plan(const g4_kv8_args* a, int32_t* cu_q, int32_t* cu_k, int32_
   if (a->window > 0) keys = std::min<int64_t>(keys, a->window);
   if (int64_t(a->batch) * (keys - 1 + a->tokens) > INT32_MAX)
     return api_fail(G4_ERR_UNSUPPORTED, "the rows' keys must fit 31 bits");
+  if (!a->holes) return api_fail(G4_ERR_INVALID, "holes is required");
   Kv8ChunkParams p;
   memset(&p, 0, sizeof(p));
   p.cache = cache_of(a);
@@ -393,6 +401,7 @@ int g4_kv8_chunk_plan(const g4_kv8_args* a, int32_t* cu_q, int32_t* cu_k, int32_
   p.cu_k = cu_k;
   p.first = first;
   p.last = last;
+  p.holes = a->holes;
   const OnDevice guard(a->device);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   LaunchScope ls(kKKv8Chunk, st);
@@ -405,15 +414,31 @@ int g4_kv8_pad_rows(const g4_kv8_args* a, void* stream) {
   if (rc) return rc;
   if ((rc = check_attn_shape(a))) return rc;
   if ((rc = check_operand(a->o, a->o_stride, "o", true))) return rc;
+  if ((rc = check_operand(a->q, a->q_stride, "q", true))) return rc;
   if (!a->lse || a->lse_stride[0] <= 0 || a->lse_stride[1] <= 0)
     return api_fail(G4_ERR_INVALID, "lse with positive strides is required");
+  if (!a->holes) return api_fail(G4_ERR_INVALID, "holes is required");
   const OnDevice guard(a->device);
+  Kv8AttnParams p = attn_of(a);
+  const int64_t columns = int64_t(p.group) * a->tokens;
+  const Kv8AttnShape shape = kv8_wide_shape(a->head_dim, columns);
+  p.cols = shape.cols;
+  p.tile = shape.tile;
+  p.col_groups = static_cast<int>((columns + shape.cols - 1) / shape.cols);
+  p.only = a->holes;
+  // one wave of CTAs: where no page is missing, more of them only come and go (2048 of
+  // them took 18 us)
+  const int64_t items = int64_t(a->num_kv_heads) * p.col_groups;
+  p.per_row = static_cast<int>(
+      std::min(items, std::max<int64_t>(1, api_sm_count() / a->batch)));
+  // (a run's operand chunks are counted in 31 bits)
+  if ((items / p.per_row + 1) * (a->max_seqlen_k / shape.tile + 2) > (int64_t(1) << 27))
+    return api_fail(G4_ERR_UNSUPPORTED, "too many (head, token, key) tiles in one row");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   LaunchScope ls(kKKv8Chunk, st);
-  return launched(launch_kv8_pad_rows(cache_of(a), rows_of(a), a->max_seqlen_k, a->num_q_heads,
-                                      a->head_dim, static_cast<__nv_bfloat16*>(a->o), a->o_stride,
-                                      a->lse, a->lse_stride, st),
-                  "padding launch");
+  return launched(launch_kv8_wide(a->head_dim, a->format == G4_KV8_INT8, p, a->batch * p.per_row,
+                                  st),
+                  "chunk completion launch");
 }
 
 size_t g4_pages_workspace_bytes(const g4_pages_args* a) { return a ? pages_work(a) : 0; }

@@ -240,6 +240,7 @@ __global__ void __launch_bounds__(128) kv8_read_kernel(const Kv8StoreParams p) {
   }
   uint2 w[2][kSteps];
   float s[2][kSteps];
+  bool hole = false;
 #pragma unroll
   for (int i = 0; i < kSteps; ++i) {
     const int pos = row.start + t0 + i * kRows + at;
@@ -252,8 +253,11 @@ __global__ void __launch_bounds__(128) kv8_read_kernel(const Kv8StoreParams p) {
       w[1][i] = __ldcs(reinterpret_cast<const uint2*>(c.v + from));
       s[0][i] = c.k_scale[block];
       s[1][i] = c.v_scale[block];
+    } else {
+      hole |= t0 + i * kRows + at < min(len, row.n);
     }
   }
+  if (hole && p.holes) p.holes[b] = 1;
 #pragma unroll
   for (int i = 0; i < kSteps; ++i) {
     const int t = t0 + i * kRows + at;
@@ -281,7 +285,9 @@ __global__ void __launch_bounds__(128) kv8_read_kernel(const Kv8StoreParams p) {
 // sees, packed: row b's queries are `tokens` rows, its keys the positions
 // [first, start + tokens), so that the queries are the keys' last rows (padding
 // included; a padded key is later than every real query).  Empty rows get
-// `tokens` zero keys; kv8_pad_rows_kernel clears their outputs.
+// `tokens` zero keys.  The bf16 kernels mask by position only: a key of a missing page
+// would count with the score of its zeros, so the read marks such rows.  The wide kernel
+// then computes the marked rows from the codes and clears the others' padding.
 __global__ void __launch_bounds__(1024) kv8_chunk_plan_kernel(const Kv8ChunkParams p) {
   __shared__ int sums[32];
   pdl_enter();
@@ -307,27 +313,9 @@ __global__ void __launch_bounds__(1024) kv8_chunk_plan_kernel(const Kv8ChunkPara
     p.cu_q[b + 1] = (b + 1) * p.rows.tokens;
     p.first[b] = first;
     p.last[b] = last;
+    p.holes[b] = 0;
   }
   if (b == 0) p.cu_q[0] = p.cu_k[0] = 0;
-}
-
-__global__ void __launch_bounds__(128) kv8_pad_rows_kernel(Kv8Cache c, Kv8Rows r, int max_k,
-                                                           __nv_bfloat16* o, int64_t os0,
-                                                           int64_t os1, int64_t os2, float* lse,
-                                                           int64_t ls0, int64_t ls1, int heads,
-                                                           int d) {
-  pdl_enter();
-  const int b = blockIdx.y;
-  const Kv8Row row = kv8_row(c, r, b, max_k);
-  for (int t = row.n + static_cast<int>(blockIdx.x); t < r.tokens; t += gridDim.x) {
-    for (int u = threadIdx.x; u < heads * d / 8; u += blockDim.x) {
-      const int h = u / (d / 8);
-      *reinterpret_cast<uint4*>(o + b * os0 + t * os1 + h * os2 + (u % (d / 8)) * 8) =
-          make_uint4(0u, 0u, 0u, 0u);
-    }
-    for (int h = threadIdx.x; h < heads; h += blockDim.x)
-      lse[b * ls0 + h * ls1 + t] = -INFINITY;
-  }
 }
 
 namespace {
@@ -370,15 +358,6 @@ int launch_kv8_read(int d, bool int8, const Kv8StoreParams& p, cudaStream_t stre
 int launch_kv8_chunk_plan(const Kv8ChunkParams& p, cudaStream_t stream) {
   return static_cast<int>(
       launch_chained(kv8_chunk_plan_kernel, dim3(1), dim3(1024), 0, stream, p));
-}
-
-int launch_kv8_pad_rows(const Kv8Cache& c, const Kv8Rows& r, int max_k, int heads, int d,
-                        __nv_bfloat16* o, const int64_t* os, float* lse, const int64_t* ls,
-                        cudaStream_t stream) {
-  const int gx = r.tokens < 64 ? r.tokens : 64;
-  return static_cast<int>(launch_chained(kv8_pad_rows_kernel, dim3(gx, r.batch), dim3(128), 0,
-                                         stream, c, r, max_k, o, os[0], os[1], os[2], lse, ls[0],
-                                         ls[1], heads, d));
 }
 
 }  // namespace g4

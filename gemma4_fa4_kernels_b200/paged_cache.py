@@ -309,12 +309,12 @@ class PagedKVCache8:
         a.k_stride[:] = a.v_stride[:] = (tokens * row, row, self.head_dim)
         return bytes(a)
 
-    def _read(self, block, batch, slots, starts, ends, k, v, out_rows) -> None:
+    def _read(self, block, batch, slots, starts, ends, k, v, out_rows, holes=None) -> None:
         a = _lib.G4Kv8Args.from_buffer_copy(block)
         self._rows(a, batch, slots, starts, ends)
         a.k, a.v = k.data_ptr(), v.data_ptr()
         if out_rows is not None:
-            a.out_rows, a.out_total = out_rows.data_ptr(), k.shape[0]
+            a.out_rows, a.out_total, a.holes = out_rows.data_ptr(), k.shape[0], holes
         self._launch(_lib.load().g4_kv8_read, ctypes.byref(a))
 
     # ----------------------------------------------------------------------------
@@ -387,21 +387,23 @@ class PagedKVCache8:
         keys = tokens + (min(max_k, window) if window else max_k) - 1  # most a row can see
         total = batch * tokens
         lib = _lib.load()
-        plan = torch.empty(4 * batch + 2, dtype=torch.int32, device=self.device)
+        plan = torch.empty(5 * batch + 2, dtype=torch.int32, device=self.device)
         cu_q, cu_k = plan[:batch + 1], plan[batch + 1:2 * batch + 2]
-        first, last = plan[2 * batch + 2:3 * batch + 2], plan[3 * batch + 2:]
+        first, last = plan[2 * batch + 2:3 * batch + 2], plan[3 * batch + 2:4 * batch + 2]
+        a.holes = plan[4 * batch + 2:].data_ptr()
         self._launch(lib.g4_kv8_chunk_plan, ctypes.byref(a), cu_q.data_ptr(), cu_k.data_ptr(),
                      first.data_ptr(), last.data_ptr())
         k = torch.empty((batch * keys, self.num_kv_heads, d), dtype=torch.bfloat16,
                         device=self.device)
         v = torch.empty_like(k)
-        self._read(self._read_block(layer, batch, keys), batch, slots, first, last, k, v, cu_k)
+        self._read(self._read_block(layer, batch, keys), batch, slots, first, last, k, v, cu_k,
+                   a.holes)
         with torch.cuda.device(self.device):
             _, lse = ops.attn_fwd(q.reshape(total, heads, d), k, v, window=window,
                                   cu_seqlens_q=cu_q, cu_seqlens_k=cu_k, max_seqlen_q=tokens,
                                   max_seqlen_k=keys, out=out.view(total, heads, d))
-        a.lse = lse.data_ptr()
-        self._launch(lib.g4_kv8_pad_rows, ctypes.byref(a))
+        a.q, a.lse = q.data_ptr(), lse.data_ptr()
+        self._launch(lib.g4_kv8_pad_rows, ctypes.byref(a))  # and rows with missing pages
         return lse.view(heads, batch, tokens).transpose(0, 1)
 
     # ----------------------------------------------------------------------------

@@ -37,7 +37,7 @@
 extern "C" {
 #endif
 
-#define G4_ABI_VERSION 2
+#define G4_ABI_VERSION 3
 
 enum g4_status {
   G4_OK = 0,
@@ -378,6 +378,8 @@ typedef struct g4_kv8_args {
                               out_rows[b + 1]) (at most `tokens` rows); batch strides unused */
   int32_t out_total;       /* packed: rows of the outputs; up to 128 behind the last segment
                               are zeroed */
+  int32_t* holes;          /* nullable, [batch]: row b's keys have a missing page.  Cleared by
+                              g4_kv8_chunk_plan, set by g4_kv8_read, read by g4_kv8_pad_rows */
   /* attention */
   const void* q; /* [batch][token][query head][head_dim] bf16 */
   void* o;
@@ -417,8 +419,10 @@ int g4_kv8_attn(const g4_kv8_args* args, void* stream);
  * layout (cu_q, cu_k: batch + 1 entries; row b's queries are its `tokens` rows,
  * its keys the positions [first[b], starts[b] + tokens)) and the positions
  * [first[b], last[b]) to read back into them (g4_kv8_read with starts = first,
- * ends = last, out_rows = cu_k); g4_kv8_pad_rows then clears the outputs of
- * padding and of empty rows.
+ * ends = last, out_rows = cu_k).  The packed forward has no mask for the keys of
+ * missing pages: g4_kv8_pad_rows computes the rows that have some, marked in `holes`
+ * (required), once more, and clears the outputs of padding and of empty rows (q, o and
+ * lse: those of the forward).
  */
 int g4_kv8_chunk_plan(const g4_kv8_args* args, int32_t* cu_q, int32_t* cu_k, int32_t* first,
                       int32_t* last, void* stream);

@@ -1,0 +1,66 @@
+"""GPU: the paged cache at the edges of what its calls serve, against the 64-bit oracle."""
+
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+if not torch.cuda.is_available():  # pragma: no cover - CPU containers
+    pytest.skip("needs a CUDA device", allow_module_level=True)
+
+from gemma4_fa4_kernels_b200.paged_cache import DIRECT_COLUMNS  # noqa: E402
+from test_gpu_paged_cache import Pair, check_attention, i32  # noqa: E402
+
+
+# ------------------------------------------------------------------------------------
+# missing pages under a chunk of a prompt
+# ------------------------------------------------------------------------------------
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("d,heads,group,window", [(512, 1, 8, 0), (512, 2, 8, 60), (256, 2, 2, 0),
+                                                 (256, 2, 4, 50), (512, 1, 3, 0)])
+def test_chunks_mask_missing_pages(fmt, d, heads, group, window):
+    rng = np.random.default_rng(41)
+    tokens = DIRECT_COLUMNS[d] // group + 3
+    lens = [tokens + 90, tokens + 40, 150, tokens + 20, tokens, 40]
+    p = Pair(fmt, heads=heads, d=d, page=16, pages=80, slots=7, per_slot=20)
+    p.fill(list(range(6)), lens, rng)
+    p.ref.tables[0, 1:3] = -1                       # a hole before the chunk
+    p.ref.tables[1, :] = -1                         # nothing at all
+    p.ref.tables[2, (lens[2] - 20) // 16] = 80      # a bad id under the chunk's own tokens
+    p.ref.tables[3, 0] = -1                         # a leading hole
+    p.ref.tables[5, (lens[5] - 1) // 16] = -1       # the last page: some queries' own keys
+    p.dev.tables.copy_(i32(p.ref.tables))
+    n = [tokens, tokens - 2, 30, tokens, tokens, 7, 0, 3]
+    rows = [0, 1, 2, 3, 4, 5, 6, 9]
+    ends = [*lens, 0, 5]
+    q = 0.2 * rng.standard_normal((8, tokens, heads * group, d))
+    poison = torch.full((1 << 25,), float("nan"), device="cuda")  # what the next buffers hold
+    del poison
+    check_attention(p, 0, q, rows, [e - m for e, m in zip(ends, n)], ends, window=window)
+
+
+def test_a_hole_means_the_same_on_both_sides_of_the_direct_bound():
+    """Three of seven pages are missing; the last 32 of 33 tokens see what 32 tokens see."""
+    rng = np.random.default_rng(42)
+    p = Pair("e4m3", heads=1, d=512, page=16, pages=12, slots=1, per_slot=12)
+    p.fill([0], [100], rng)
+    p.ref.tables[0, 1:4] = -1
+    p.dev.tables.copy_(i32(p.ref.tables))
+    q = 0.05 * rng.standard_normal((1, 33, 8, 512))
+    many = check_attention(p, 0, q, [0], [67], [100])
+    few = check_attention(p, 0, q[:, 1:], [0], [68], [100])
+    # BF16 outputs (2^-8 of each) and a chunk's P (2^-7 of sum p |v|, which is up to 1.5 max)
+    assert np.abs(many[:, 1:] - few).max() <= 2.0 ** -5 * np.abs(few).max()
+
+
+def test_a_chunk_over_trimmed_pages():
+    """Positions that are run again after a trim see what is left."""
+    rng = np.random.default_rng(43)
+    p = Pair("int8", heads=2, d=256, page=16, pages=40, slots=2, per_slot=20)
+    p.fill([0, 1], [250, 100], rng)
+    p.ref.free([0], 100)
+    p.dev.trim(i32([0]), 100)
+    q = 0.2 * rng.standard_normal((2, 80, 4, 256))
+    check_attention(p, 0, q, [0, 1], [170, 20], [250, 100], window=140)
+    p.same()
