@@ -768,8 +768,10 @@ template <typename Cfg, bool kInt8>
 int launch_wide(const Kv8AttnParams& p, int ctas, cudaStream_t stream) {
   static_assert(Cfg::smem(kKv8MaxBatch) <= kKv8MaxSmem, "shared memory of the largest batch");
   const int smem = Cfg::smem(p.rows.batch);
+  // a property of the kernel and not of the call: the same from every host thread
   cudaError_t e = cudaFuncSetAttribute(kv8_wide_kernel<Cfg, kInt8>,
-                                       cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+                                       cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                       Cfg::smem(kKv8MaxBatch));
   if (e == cudaSuccess)
     e = launch_chained(kv8_wide_kernel<Cfg, kInt8>, dim3(ctas), dim3(kWideThreads), smem, stream,
                        p);

@@ -1,5 +1,7 @@
 """GPU: the paged cache at the edges of what its calls serve, against the 64-bit oracle."""
 
+import threading
+
 import numpy as np
 import pytest
 import torch
@@ -9,8 +11,9 @@ pytestmark = pytest.mark.gpu
 if not torch.cuda.is_available():  # pragma: no cover - CPU containers
     pytest.skip("needs a CUDA device", allow_module_level=True)
 
+from gemma4_fa4_kernels_b200 import PagedKVCache8  # noqa: E402
 from gemma4_fa4_kernels_b200.paged_cache import DIRECT_COLUMNS  # noqa: E402
-from test_gpu_paged_cache import Pair, check_attention, i32  # noqa: E402
+from test_gpu_paged_cache import Pair, bf16, check_attention, i32  # noqa: E402
 
 
 # ------------------------------------------------------------------------------------
@@ -64,3 +67,45 @@ def test_a_chunk_over_trimmed_pages():
     q = 0.2 * rng.standard_normal((2, 80, 4, 256))
     check_attention(p, 0, q, [0, 1], [170, 20], [250, 100], window=140)
     p.same()
+
+
+# ------------------------------------------------------------------------------------
+# host threads
+# ------------------------------------------------------------------------------------
+@pytest.mark.parametrize("tokens", [1, 5])
+def test_host_threads_with_batches_of_different_size(tokens):
+    """Calls of one kernel from six host threads, 1024 rows in three, one in the others."""
+    caches, args = [], []
+    for rows in (1024, 1):
+        cache = PagedKVCache8(1, rows, 1, 512, max_slots=rows, pages_per_slot=100, page_size=16)
+        slots = i32(range(rows))
+        starts, ends = cache.extend(slots, i32([7] * rows))
+        k, _ = bf16(np.ones((rows, 7, 1, 512)))
+        cache.append(0, k, k.clone(), slots, starts, ends)
+        q, _ = bf16(0.01 * np.ones((rows, tokens, 8, 512)))
+        caches.append(cache)
+        args.append((0, q, slots, ends - tokens, ends))
+    want = [c.attention(*a) for c, a in zip(caches, args)]
+    torch.cuda.synchronize()
+    errors, last = [], [None] * 6
+    go = threading.Barrier(6)
+
+    def work(i):
+        try:
+            stream = torch.cuda.Stream()
+            go.wait(30)
+            with torch.cuda.stream(stream):
+                for _ in range(3000):  # no waits: the launch queue is full
+                    last[i] = caches[i % 2].attention(*args[i % 2])
+        except Exception as e:  # noqa: BLE001
+            errors.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(6)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not errors, errors[0]
+    for i, (out, lse) in enumerate(last):
+        assert torch.equal(out, want[i % 2][0]) and torch.equal(lse, want[i % 2][1])
