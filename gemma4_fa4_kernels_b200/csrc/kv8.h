@@ -13,7 +13,8 @@
 // A table row lists the pages of one sequence in order, -1 where there is none.
 // Rows, page ids and positions that the device arrays carry are checked where
 // they are used: an out-of-range page is never read or written (its keys count
-// as masked), and a row whose slot or positions are out of range counts as empty.
+// as masked), and a row whose slot or positions are out of range counts as empty and is
+// reported.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -63,22 +64,29 @@ struct Kv8Rows {
 };
 
 struct Kv8Row {
-  int slot;                 // -1: empty row
+  int slot;                 // -1: asks for nothing, kKv8BadRow: for what is out of range
   int start;
   int n;                    // tokens of the row, <= rows.tokens
 };
 
-// Checked row b: empty (slot -1, n 0) when its slot or positions are out of range.
+constexpr int kKv8BadRow = -2;
+
+// Checked row b: empty (n 0) when its slot or positions are out of range.
 __device__ __forceinline__ Kv8Row kv8_row(const Kv8Cache& c, const Kv8Rows& r, int b, int max_end) {
   Kv8Row o;
   const int slot = r.slots ? r.slots[b] : b;
   const int start = r.starts[b], end = r.ends[b];
   const bool ok = slot >= 0 && slot < c.num_slots && start >= 0 && end > start && end <= max_end &&
                   (end - 1) >> c.page_shift < c.pages_per_slot;
-  o.slot = ok ? slot : -1;
+  o.slot = ok ? slot : end > start ? kKv8BadRow : -1;
   o.start = ok ? start : 0;
   o.n = ok ? min(end - start, r.tokens) : 0;
   return o;
+}
+
+// Reports a row of a call (one thread of the launch).
+__device__ __forceinline__ void kv8_report(int* status, int slot) {
+  if (slot == kKv8BadRow && status) atomicOr(status, kKv8BadIndex);
 }
 
 // Page of a position; -1 when there is none.
@@ -179,6 +187,7 @@ struct Kv8ChunkParams {
   int* first;               // [batch] first key read
   int* last;                // [batch] one past the last key read
   int* holes;               // [batch] cleared
+  int* status;              // nullable
 };
 int launch_kv8_chunk_plan(const Kv8ChunkParams& p, cudaStream_t stream);
 

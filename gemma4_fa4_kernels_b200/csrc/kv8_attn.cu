@@ -135,7 +135,10 @@ __global__ void __launch_bounds__(Cfg::kThreads, 1) kv8_attn_kernel(const Kv8Att
   int todo = 0;
   if (p.whole) {  // the CTA's item, cut into a run per team
     const int items = heads * p.col_groups, b = blockIdx.x / items;
-    if (tid == 0) rows[b] = row_plan(p, b);
+    if (tid == 0) {
+      rows[b] = row_plan(p, b);
+      if (blockIdx.x == b * items) kv8_report(p.status, rows[b].slot);
+    }
     __syncthreads();
     first = list.item_place(b, blockIdx.x - b * items);
     const int runs = min(first.left, Cfg::kTeams);

@@ -323,6 +323,7 @@ int g4_kv8_read(const g4_kv8_args* a, void* stream) {
   p.out_rows = a->out_rows;
   p.out_total = a->out_total;
   p.holes = a->holes;
+  p.status = a->status;
   const OnDevice guard(a->device);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   LaunchScope ls(kKKv8Read, st);
@@ -402,6 +403,7 @@ int g4_kv8_chunk_plan(const g4_kv8_args* a, int32_t* cu_q, int32_t* cu_k, int32_
   p.first = first;
   p.last = last;
   p.holes = a->holes;
+  p.status = a->status;
   const OnDevice guard(a->device);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   LaunchScope ls(kKKv8Chunk, st);

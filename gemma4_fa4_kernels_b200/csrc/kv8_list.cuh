@@ -147,7 +147,7 @@ struct TileList {
 };
 
 // The whole CTA: prefix sums of the rows' weights, and the plan that the merge reads
-// (written by CTA 0).  `keep(b, row)` sees every row once, before `rows(b)` is used.
+// (written by CTA 0, which also reports the rows).  `keep(b, row)` sees every row once, before `rows(b)` is used.
 template <int kThreads, typename List, typename Keep>
 __device__ __forceinline__ void plan_rows(const Kv8AttnParams& p, const List& list, int* prefix,
                                           int* scan, const Keep& keep) {
@@ -159,8 +159,10 @@ __device__ __forceinline__ void plan_rows(const Kv8AttnParams& p, const List& li
     if (b >= B) break;
     const RowPlan r = row_plan(p, b);
     keep(b, r);
-    if (blockIdx.x == 0)
+    if (blockIdx.x == 0) {
       reinterpret_cast<int4*>(p.plan)[1 + b] = make_int4(r.slot, r.start, r.n, r.lo);
+      kv8_report(p.status, r.slot);
+    }
     mine += list.row_weight(r);
   }
   int inc = mine;

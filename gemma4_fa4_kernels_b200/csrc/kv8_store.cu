@@ -98,7 +98,10 @@ __global__ void __launch_bounds__(512) kv8_append_kernel(const Kv8StoreParams p)
   const int head = blockIdx.y;
   const Kv8Cache& c = p.cache;
   const Kv8Row row = kv8_row(c, p.rows, b, INT32_MAX);
-  if (row.n <= 0) return;
+  if (row.n <= 0) {
+    if (blockIdx.x == 0 && head == 0 && !is_v && threadIdx.x == 0) kv8_report(p.status, row.slot);
+    return;
+  }
   const int first = row.start >> c.page_shift;
   const int page_pos = (first + static_cast<int>(blockIdx.x)) << c.page_shift;
   const int a = max(row.start, page_pos);
@@ -220,6 +223,7 @@ __global__ void __launch_bounds__(128) kv8_read_kernel(const Kv8StoreParams p) {
   const int head = blockIdx.y;
   const Kv8Cache& c = p.cache;
   const Kv8Row row = kv8_row(c, p.rows, b, INT32_MAX);
+  if (blockIdx.x == 0 && head == 0 && threadIdx.x == 0) kv8_report(p.status, row.slot);
   const int base = p.out_rows ? p.out_rows[b] : 0;
   int len = p.out_rows ? p.out_rows[b + 1] - base : p.rows.tokens;
   if (p.out_rows && b == p.rows.batch - 1) len += min(kReadTail, p.out_total - base - len);
@@ -295,6 +299,7 @@ __global__ void __launch_bounds__(1024) kv8_chunk_plan_kernel(const Kv8ChunkPara
   int keys = 0, first = 0, last = 0;
   if (b < p.rows.batch) {
     const Kv8Row r = kv8_row(p.cache, p.rows, b, p.max_k);
+    kv8_report(p.status, r.slot);
     first = p.window > 0 ? max(0, r.start - p.window + 1) : 0;
     keys = r.start + p.rows.tokens - first;
     last = r.start + r.n;

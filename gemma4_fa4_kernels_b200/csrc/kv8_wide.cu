@@ -218,6 +218,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv8_wide_kernel(const Kv8Attn
   int todo = 0;
   if (p.whole) {
     const int items = heads * p.col_groups, b = W / items;
+    if (W == b * items && tid == 0) kv8_report(p.status, row_at(b).slot);
     __syncthreads();
     pl = list.item_place(b, W - b * items);
     todo = pl.left;

@@ -25,7 +25,8 @@ A step of a batch::
 ``starts``/``ends`` (int32, one per row) are the positions of the row's tokens.
 Operands are padded batches ``(rows, tokens, heads, head_dim)``: row b uses its
 first ``ends[b] - starts[b]`` tokens, outputs of padding are zero (LSE -inf).  A
-row whose slot or positions are out of range counts as empty; a row that
+row with ``ends[b] <= starts[b]`` asks for nothing, whatever its slot.  One that
+asks for a slot or positions out of range counts as empty; a row that
 :meth:`extend`, :meth:`fork` or :meth:`copy_pages` cannot serve is left as it was.
 Both raise a bit of ``status``, which :meth:`check` turns into an exception.
 Slots of one call must be distinct.
@@ -329,7 +330,7 @@ class PagedKVCache8:
         Returns ``(out, lse)``: BF16 of q's shape and float32 (rows, query heads,
         tokens); zeros and -inf for padding and for a query without a visible key.
         ``max_seqlen_k`` (default: a slot's capacity) bounds ``ends``; a tighter bound
-        sizes the launch and its buffers better, and a row beyond it counts as empty.
+        sizes the launch and its buffers better; a row beyond it is out of range.
         """
         key = ("attention", layer, window, max_seqlen_k, q.shape, q.stride(), q.dtype, q.device)
         call = self._calls.get(key) or self._attention_call(key, layer, q, window, max_seqlen_k)

@@ -342,10 +342,11 @@ int g4_prep_bwd(const g4_prep_args* args, void* stream);
  * A call serves `batch` rows.  Row b uses table row slots[b] (b itself when slots
  * is null), its tokens sit at positions starts[b] .. ends[b] - 1, and they are the
  * first min(ends[b] - starts[b], tokens) of its `tokens` rows in the operands; the
- * rest is padding.  A row with ends[b] <= starts[b], or whose slot or positions
- * are out of range, is empty.  These arrays are read on the device.  At most 1024
- * rows; page sizes 16, 32, 64 and 128; head dims 256 and 512; operand strides in
- * elements, multiples of 8; 16-byte aligned bases.
+ * rest is padding.  A row with ends[b] <= starts[b] is empty, and so is one whose
+ * slot or positions are out of range, which raises G4_PAGES_BAD_INDEX in *status.
+ * These arrays are read on the device.  At most 1024 rows; page sizes 16, 32, 64
+ * and 128; head dims 256 and 512; operand strides in elements, multiples of 8;
+ * 16-byte aligned bases.
  */
 enum g4_kv8_format { G4_KV8_E4M3 = 0, G4_KV8_INT8 = 1 };
 typedef struct g4_kv8_args {
@@ -389,7 +390,7 @@ typedef struct g4_kv8_args {
   int64_t lse_stride[2]; /* batch, head */
   int32_t num_q_heads;
   int32_t window;       /* 0: every earlier key; W > 0: keys k > position - W */
-  int32_t max_seqlen_k; /* upper bound of ends; a row beyond it is empty */
+  int32_t max_seqlen_k; /* upper bound of ends; a row beyond it is out of range */
   int32_t device;       /* CUDA device of the pointers and the stream; -1: the current one */
   void* workspace;
   size_t workspace_bytes;

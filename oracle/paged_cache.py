@@ -48,9 +48,13 @@ class PagedCache:
 
     # -- rows ---------------------------------------------------------------------
     def _row(self, slot, start, end, tokens, max_end=1 << 40):
-        ok = (0 <= slot < len(self.lengths) and 0 <= start < end <= max_end
-              and (end - 1) // self.page < self.tables.shape[1])
-        return min(end - start, tokens) if ok else 0
+        if end <= start:
+            return 0  # asks for nothing
+        if (0 <= slot < len(self.lengths) and 0 <= start and end <= max_end
+                and (end - 1) // self.page < self.tables.shape[1]):
+            return min(end - start, tokens)
+        self.status |= BAD_INDEX
+        return 0
 
     def _page(self, slot, pos):
         p = self.tables[slot, pos // self.page]

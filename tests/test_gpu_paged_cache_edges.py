@@ -11,9 +11,11 @@ pytestmark = pytest.mark.gpu
 if not torch.cuda.is_available():  # pragma: no cover - CPU containers
     pytest.skip("needs a CUDA device", allow_module_level=True)
 
-from gemma4_fa4_kernels_b200 import PagedKVCache8  # noqa: E402
+from gemma4_fa4_kernels_b200 import PagedKVCache8, _lib  # noqa: E402
 from gemma4_fa4_kernels_b200.paged_cache import DIRECT_COLUMNS  # noqa: E402
 from test_gpu_paged_cache import Pair, bf16, check_attention, i32  # noqa: E402
+
+BAD = _lib.G4_PAGES_BAD_INDEX
 
 
 # ------------------------------------------------------------------------------------
@@ -67,6 +69,66 @@ def test_a_chunk_over_trimmed_pages():
     q = 0.2 * rng.standard_normal((2, 80, 4, 256))
     check_attention(p, 0, q, [0, 1], [170, 20], [250, 100], window=140)
     p.same()
+
+
+# ------------------------------------------------------------------------------------
+# rows out of range
+# ------------------------------------------------------------------------------------
+def _calls(p, tokens_of):
+    """Every call that takes rows, at its direct, wide and chunk sizes."""
+    d, h = p.ref.k.shape[4], p.ref.k.shape[2]
+
+    def append(rows):
+        k, _ = bf16(np.ones((len(rows[0]), 3, h, d)))
+        p.dev.append(0, k, k.clone(), *map(i32, rows))
+
+    def read(rows):
+        k, v = p.dev.read(0, *map(i32, rows), 3)
+        assert not k[1].any() and not v[1].any()
+
+    def attention(rows, tokens, **kw):
+        q, _ = bf16(np.ones((len(rows[0]), tokens, 2 * h, d)))
+        out, lse = p.dev.attention(0, q, *map(i32, rows), **kw)
+        assert not out[1].any() and torch.isneginf(lse[1]).all()
+
+    calls = {"append": append, "read": read}
+    for name, tokens in tokens_of.items():
+        calls[name] = lambda rows, t=tokens, **kw: attention(rows, t, **kw)
+    return calls
+
+
+@pytest.mark.parametrize("call", ["append", "read", "decode", "wide", "chunk"])
+@pytest.mark.parametrize("per_slot", [2, 60])
+def test_rows_out_of_range_are_reported(call, per_slot):
+    """Row 1 of two: a bad slot, a negative position, a position past the table."""
+    p = Pair("int8", heads=1, d=256, page=16, pages=8, slots=3, per_slot=per_slot)
+    p.extend([0, 1, 2], [20, 20, 20])
+    run = _calls(p, {"decode": 1, "wide": 9, "chunk": 40})[call]
+    cap = 16 * per_slot
+    for slot, start, end in ((-1, 0, 3), (3, 0, 1), (1 << 30, 5, 7), (1, -1, 1), (1, -5, -4),
+                             (1, cap - 1, cap + 1), (1, cap, cap + 2), (2, 0, 2 ** 31 - 1)):
+        assert int(p.dev.status.item()) == 0
+        run(([0, slot], [0, start], [1, end]))
+        assert int(p.dev.status.item()) == BAD, (slot, start, end)
+        with pytest.raises(RuntimeError, match="out of range"):
+            p.dev.check()
+    # a row that asks for nothing is none of these, whatever its slot
+    for slot, start, end in ((1, 4, 4), (1, 0, 0), (-1, 0, 0), (9, 7, 7), (1, 5, 2)):
+        run(([0, slot], [0, start], [1, end]))
+        p.dev.check()
+
+
+@pytest.mark.parametrize("tokens", [1, 9, 40])
+def test_rows_beyond_the_bound_of_a_call_are_reported(tokens):
+    p = Pair("e4m3", heads=1, d=256, page=16, pages=12, slots=2, per_slot=60)
+    p.fill([0, 1], [60, 60], np.random.default_rng(44))
+    run = _calls(p, {"a": tokens})["a"]
+    run(([0, 1], [9, 50], [10, 51]), max_seqlen_k=50)
+    with pytest.raises(RuntimeError, match="out of range"):
+        p.dev.check()
+    q, _ = bf16(np.ones((2, tokens, 2, 256)))
+    p.dev.attention(0, q, i32([0, 1]), i32([9, 49]), i32([10, 50]), max_seqlen_k=50)
+    p.dev.check()
 
 
 # ------------------------------------------------------------------------------------
