@@ -22,14 +22,16 @@ namespace {
 
 constexpr int kPlanThreads = 1024;
 
-// Inclusive scan over the block's 1024 threads; `total` is the last value.
+// Inclusive scan over the block's 1024 threads; `total` is the last value.  Sums stop at
+// kMost, which is more than any pool's pages: 1024 rows may ask for 2^27 each.
+constexpr int kMost = 1 << 29;
 __device__ __forceinline__ int block_scan(int v, int* sums, int* total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int inc = v;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const int up = __shfl_up_sync(0xffffffffu, inc, o);
-    if (lane >= o) inc += up;
+    if (lane >= o) inc = min(inc + up, kMost);
   }
   __syncthreads();  // sums may hold an earlier scan
   if (lane == 31) sums[warp] = inc;
@@ -39,13 +41,13 @@ __device__ __forceinline__ int block_scan(int v, int* sums, int* total) {
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int up = __shfl_up_sync(0xffffffffu, s, o);
-      if (lane >= o) s += up;
+      if (lane >= o) s = min(s + up, kMost);
     }
     sums[lane] = s;
   }
   __syncthreads();
   *total = sums[31];
-  return warp > 0 ? inc + sums[warp - 1] : inc;
+  return warp > 0 ? min(inc + sums[warp - 1], kMost) : inc;
 }
 
 // Each warp owns a run of pages in order, each step of it 32 consecutive ones:
@@ -155,11 +157,24 @@ __global__ void __launch_bounds__(kPlanThreads) pages_extend_kernel(const Kv8Pag
     }
   }
   int total;
-  const int inc = block_scan(need, sums, &total);
+  int inc = block_scan(need, sums, &total);
   const int n_free = total > 0 ? count_free(p.refcounts, p.num_pages, sums) : 0;
-  if (ok && need > 0 && inc > n_free) {
-    ok = false;
-    raise(p.status, kKv8PoolExhausted);
+  if (total > n_free) {  // not for all: a row that finds too few leaves them to those behind it
+    if (b < p.batch) first[b] = need;
+    __syncthreads();
+    if (b == 0) {
+      for (int j = 0, left = n_free; j < p.batch; ++j) {
+        const int n = first[j];
+        if (n <= left) left -= n; else first[j] = -1;
+      }
+    }
+    __syncthreads();
+    if (b < p.batch && first[b] < 0) {
+      ok = false;
+      need = 0;
+      raise(p.status, kKv8PoolExhausted);
+    }
+    inc = block_scan(need, sums, &total);
   }
   if (b < p.batch) {
     first[b] = inc - need;

@@ -413,8 +413,9 @@ class PagedKVCache8:
     def extend(self, slots: torch.Tensor, counts):
         """Reserve pages for ``counts`` (int32 per row, or one int) more tokens of each
         slot and advance its length.  Returns ``(starts, ends)``, the new tokens'
-        positions; a row that does not fit (its table is full, the pool is empty, its
-        slot is bad or listed before) is left as it was with start = end."""
+        positions; a row that does not fit (its table is full, the pool has too few
+        pages left by the rows before it, its slot is bad or listed before) is left as
+        it was with start = end."""
         batch = self._page_rows(slots, "slots")
         if isinstance(counts, int):
             counts = torch.full((batch,), counts, dtype=torch.int32, device=self.device)
@@ -482,7 +483,7 @@ class PagedKVCache8:
         if bits:
             self.status.zero_()
             what = [text for bit, text in (
-                (_lib.G4_PAGES_EXHAUSTED, "no free page was left"),
+                (_lib.G4_PAGES_EXHAUSTED, "too few free pages were left"),
                 (_lib.G4_PAGES_ROW_FULL, "a slot's table was full"),
                 (_lib.G4_PAGES_BAD_INDEX, "a slot, page or count was out of range or listed twice"),
                 (_lib.G4_KV8_DEVICE_WAIT, "a kernel's bounded wait expired (invalid results)"),

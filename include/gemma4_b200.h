@@ -434,9 +434,9 @@ int g4_kv8_pad_rows(const g4_kv8_args* args, void* stream);
  * call reads it back.  lengths[slot]: tokens; refcounts[page]: tables that list
  * the page (0 = free).  Pages are taken from the lowest free ids in order of the
  * rows.  A row that cannot be served is left as it was and raises a bit of *status:
- * G4_PAGES_EXHAUSTED no free page (rows are served in order until the pool is
- * empty), G4_PAGES_ROW_FULL its table is full, G4_PAGES_BAD_INDEX an index out of
- * range or listed twice.
+ * G4_PAGES_EXHAUSTED too few free pages (rows are served in order; one that finds
+ * too few leaves them to the rows behind it), G4_PAGES_ROW_FULL its table is full,
+ * G4_PAGES_BAD_INDEX an index out of range or listed twice.
  */
 #define G4_PAGES_EXHAUSTED 1
 #define G4_PAGES_ROW_FULL 2

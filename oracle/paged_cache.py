@@ -144,7 +144,6 @@ class PagedCache:
 
     def extend(self, slots, counts):
         starts, ends = np.zeros(len(slots), int), np.zeros(len(slots), int)
-        wanted = 0
         free = [p for p in range(len(self.refcounts)) if self.refcounts[p] == 0]
         for b, (s, n) in enumerate(zip(slots, counts)):
             if self._slot(s):
@@ -160,13 +159,13 @@ class PagedCache:
                 self.status |= ROW_FULL
                 continue
             have, want = -(-self.lengths[s] // self.page), -(-new // self.page)
-            at, wanted = wanted, wanted + want - have
-            if want > have and wanted > len(free):
+            if want - have > len(free):
                 self.status |= EXHAUSTED
                 continue
             for j in range(want - have):
-                self.tables[s, have + j] = free[at + j]
-                self.refcounts[free[at + j]] = 1
+                page = free.pop(0)
+                self.tables[s, have + j] = page
+                self.refcounts[page] = 1
             self.lengths[s] = ends[b] = new
         return starts, ends
 

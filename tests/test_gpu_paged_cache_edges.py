@@ -132,6 +132,53 @@ def test_rows_beyond_the_bound_of_a_call_are_reported(tokens):
 
 
 # ------------------------------------------------------------------------------------
+# a pool that runs out
+# ------------------------------------------------------------------------------------
+def test_a_refused_row_leaves_its_pages_to_the_rows_behind_it():
+    p = Pair("int8", pages=5, slots=6, per_slot=12, page=16)
+    p.extend([0, 1], [160, 16])                 # ten pages are not there, one is
+    assert p.ref.lengths.tolist() == [0, 16, 0, 0, 0, 0]
+    assert p.ref.status == _lib.G4_PAGES_EXHAUSTED
+    p.same()
+    p.extend([2, 3, 0, 4, 5], [70, 48, 33, 0, 16])   # 5, 3, 3, 0, 1 of four free pages
+    assert p.ref.lengths.tolist() == [0, 16, 0, 48, 0, 16]
+    p.same()
+
+
+@pytest.mark.parametrize("seed", range(6))
+def test_a_scarce_pool_serves_what_fits_in_order(seed):
+    rng = np.random.default_rng(70 + seed)
+    rows = int(rng.choice([3, 33, 200, 1024]))
+    p = Pair("int8", heads=1, pages=int(rng.integers(1, 2 * rows)), slots=rows, per_slot=6, page=16,
+             seed=seed)
+    for _ in range(4):
+        order = rng.permutation(rows)[:int(rng.integers(1, rows + 1))]
+        p.extend(list(order), list(rng.integers(0, 50, len(order))))
+        p.same()
+        gone = rng.choice(rows, max(1, rows // 4), replace=False)
+        p.ref.free(list(gone))
+        p.dev.free(i32(gone))
+    p.same()
+
+
+def test_rows_that_ask_for_more_than_31_bits_of_pages_together():
+    per_slot, rows = (2 ** 31 - 1 - 65536) // 16, 17
+    tables = torch.full((rows, per_slot), -1, dtype=torch.int32, device="cuda")
+    codes = [torch.zeros(1, 3, 1, 16, 256, dtype=torch.int8, device="cuda") for _ in range(2)]
+    scales = [torch.ones(1, 3, 1, device="cuda") for _ in range(2)]
+    cache = PagedKVCache8.from_tensors(*codes, *scales, tables, i32([0] * rows), i32([0] * 3))
+    counts = [16 * per_slot] * (rows - 1) + [33]
+    starts, ends = cache.extend(i32(range(rows)), i32(counts))
+    assert starts.tolist() == [0] * rows and ends.tolist() == [0] * (rows - 1) + [33]
+    assert cache.lengths.tolist() == ends.tolist()
+    assert cache.refcounts.tolist() == [1, 1, 1] and tables[-1, :4].tolist() == [0, 1, 2, -1]
+    with pytest.raises(RuntimeError, match="too few free pages"):
+        cache.check()
+    del tables, cache
+    torch.cuda.empty_cache()
+
+
+# ------------------------------------------------------------------------------------
 # host threads
 # ------------------------------------------------------------------------------------
 @pytest.mark.parametrize("tokens", [1, 5])
