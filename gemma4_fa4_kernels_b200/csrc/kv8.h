@@ -27,11 +27,13 @@ namespace g4 {
 constexpr int kKv8MaxBatch = 1024;  // rows of one call (their plan sits in shared memory)
 constexpr int kKv8MaxSmem = 232448; // dynamic shared memory per CTA
 constexpr int kKv8Tile = 32;        // keys per attention tile: two pieces of 16, each in one page
-// exponents of a block's scale 2^e: 2^e and 2^-e are both normal fp32 values, and
-// the largest finite bf16 value fits 448 * 2^120 and 127 * 2^122
+// Exponents of a block's scale 2^e: 2^e and 2^-e are both normal fp32 values, and every
+// code * scale is finite in fp32 and bf16.  The largest bf16 value is 255 * 2^120 or
+// 127.5 * 2^121: at the largest exponent codes stop at 240 (e4m3, whose next one is 256)
+// and 127 (int8), off by at most 2^-4 of the value and half a step, as everywhere.
 constexpr int kKv8MinExp = -100;
-constexpr int kKv8MaxExp = 122;
-
+template <bool kInt8>
+constexpr int kKv8MaxExp = kInt8 ? 121 : 120;
 
 enum Kv8Status : int {
   kKv8PoolExhausted = 1,    // no free page left for a row

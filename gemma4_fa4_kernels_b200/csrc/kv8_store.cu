@@ -4,7 +4,7 @@
 // Append.  A block (page, KV head) has the scale 2^e with the least e such that
 // its largest finite magnitude is at most `top` * 2^e (448 for e4m3, 127 for
 // int8), e in [kKv8MinExp, kKv8MaxExp]:
-//   code = round_to_nearest_even(x * 2^-e).
+//   code = round_to_nearest_even(x * 2^-e), at the largest e at most 240 (e4m3).
 // When tokens join a page that holds earlier ones, e only grows; the older codes
 // are then requantised from their own values.  x * 2^-e is exact (a power of
 // two), so the one rounding is the format's.  Codes are always finite: infinities
@@ -34,14 +34,14 @@ __device__ __forceinline__ int block_exponent(uint32_t bits) {  // bits: bf16 ma
   // magnitude 1.f * 2^(x - 127); top = 1.75 * 2^8 (e4m3) or 1.984375 * 2^6 (int8)
   const int x = static_cast<int>(bits >> 7), f = static_cast<int>(bits & 127u);
   const int e = kInt8 ? x - 127 - 6 + (f > 126) : x - 127 - 8 + (f > 96);
-  return bits == 0 ? kKv8MinExp : min(max(e, kKv8MinExp), kKv8MaxExp);
+  return bits == 0 ? kKv8MinExp : min(max(e, kKv8MinExp), kKv8MaxExp<kInt8>);
 }
 
 __device__ __forceinline__ float pow2f(int e) {  // -126 <= e <= 127
   return __uint_as_float(static_cast<uint32_t>(e + 127) << 23);
 }
 
-// Codes of four finite values that the block's scale covers.
+// Codes of four finite values that the block's scale covers (below the largest scale).
 template <bool kInt8>
 __device__ __forceinline__ uint32_t pack4_fast(float a, float b, float c, float d, float back) {
   if constexpr (kInt8) {
@@ -60,18 +60,18 @@ __device__ __forceinline__ uint32_t pack4_fast(float a, float b, float c, float 
   }
 }
 
-// The same for any values: infinities saturate, NaN becomes 0.
+// The same for any values: what lies beyond `top` saturates, NaN becomes 0.
 template <bool kInt8>
-__device__ __forceinline__ uint32_t pack4(float a, float b, float c, float d) {
+__device__ __forceinline__ uint32_t pack4(float a, float b, float c, float d, float top) {
   if constexpr (kInt8) {
-    const auto code = [](float x) {
-      const float y = x == x ? fminf(fmaxf(x, -127.f), 127.f) : 0.f;
+    const auto code = [&](float x) {
+      const float y = x == x ? fminf(fmaxf(x, -top), top) : 0.f;
       return static_cast<uint32_t>(__float2int_rn(y)) & 255u;
     };
     return code(a) | (code(b) << 8) | (code(c) << 16) | (code(d) << 24);
   } else {
-    const auto fin = [](float x) { return x == x ? x : 0.f; };
-    uint16_t lo, hi;  // satfinite: infinities to +-448; the first source is the upper byte
+    const auto fin = [&](float x) { return x == x ? fminf(fmaxf(x, -top), top) : 0.f; };
+    uint16_t lo, hi;  // the first source is the upper byte
     asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(fin(b)), "f"(fin(a)));
     asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(fin(d)), "f"(fin(c)));
     return static_cast<uint32_t>(lo) | (static_cast<uint32_t>(hi) << 16);
@@ -161,13 +161,16 @@ __global__ void __launch_bounds__(512) kv8_append_kernel(const Kv8StoreParams p)
   __syncthreads();
   for (int w = 0; w < static_cast<int>(blockDim.x >> 5); ++w) m = max(m, red[w]);
   int e = block_exponent<kInt8>(m);
+  const auto top_code = [](int exp) {
+    return kInt8 ? 127.f : exp == kKv8MaxExp<kInt8> ? 240.f : 448.f;
+  };
   if (held > 0) {
     // least power of two not below the stored scale (which is one itself when the
     // append wrote it)
     const uint32_t ob = __float_as_uint(old_scale);
     const int oe = static_cast<int>((ob >> 23) & 255u) - 127 + ((ob & 0x7fffffu) != 0);
-    e = max(e, min(max(oe, kKv8MinExp), kKv8MaxExp));
-    const float back = pow2f(-e);
+    e = max(e, min(max(oe, kKv8MinExp), kKv8MaxExp<kInt8>));
+    const float back = pow2f(-e), top = top_code(e);
     if (old_scale * back != 1.f) {
       for (int u = threadIdx.x; u < held * kPerRow; u += blockDim.x) {
         uint2* at = reinterpret_cast<uint2*>(codes + static_cast<int64_t>(u) * kChunk);
@@ -179,13 +182,14 @@ __global__ void __launch_bounds__(512) kv8_append_kernel(const Kv8StoreParams p)
           kv8_to_half<kInt8>(w[i], lo, hi);
           const float2 l2 = half2_floats(lo), h2 = half2_floats(hi);
           w[i] = pack4<kInt8>(l2.x * old_scale * back, l2.y * old_scale * back,
-                              h2.x * old_scale * back, h2.y * old_scale * back);
+                              h2.x * old_scale * back, h2.y * old_scale * back, top);
         }
         *at = make_uint2(w[0], w[1]);
       }
     }
   }
-  const float back = pow2f(-e);
+  const float back = pow2f(-e), top = top_code(e);
+  const bool any = odd || e == kKv8MaxExp<kInt8>;  // values beyond the codes
   codes += static_cast<int64_t>(held) * D;
 #pragma unroll
   for (int s = 0; s < kSteps; ++s) {
@@ -200,7 +204,7 @@ __global__ void __launch_bounds__(512) kv8_append_kernel(const Kv8StoreParams p)
                             __uint_as_float(r[2 * i] & 0xffff0000u),
                             __uint_as_float(r[2 * i + 1] << 16),
                             __uint_as_float(r[2 * i + 1] & 0xffff0000u)};
-        w[i] = odd ? pack4<kInt8>(v[0] * back, v[1] * back, v[2] * back, v[3] * back)
+        w[i] = any ? pack4<kInt8>(v[0] * back, v[1] * back, v[2] * back, v[3] * back, top)
                    : pack4_fast<kInt8>(v[0], v[1], v[2], v[3], back);
       }
       *reinterpret_cast<uint2*>(codes + static_cast<int64_t>(u) * kChunk) = make_uint2(w[0], w[1]);

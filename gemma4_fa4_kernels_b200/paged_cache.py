@@ -8,7 +8,7 @@ element in one byte:
   [token][head_dim]`` codes, ``torch.float8_e4m3fn`` or ``torch.int8``;
 * a block (one page of one KV head) has one float32 scale, value = code * scale.
   :meth:`PagedKVCache8.append` chooses powers of two: the least one that holds
-  the block's largest magnitude.  Codes are finite (infinities saturate, NaN
+  the block's largest magnitude.  Values are finite (infinities saturate, NaN
   becomes 0);
 * ``tables`` (slots, pages per slot) lists each sequence's pages, -1 where there
   is none; ``lengths`` (slots) counts its tokens; ``refcounts`` (pages) says how
@@ -103,8 +103,9 @@ class PagedKVCache8:
     def from_tensors(cls, k, v, k_scale, v_scale, tables, lengths, refcounts) -> "PagedKVCache8":
         """A cache over existing tensors (kept, not copied): codes ``k``, ``v``
         (layers, pages, KV heads, page_size, head_dim), scales ``k_scale``,
-        ``v_scale`` (layers, pages, KV heads) float32, ``tables`` (slots,
-        pages per slot), ``lengths`` (slots) and ``refcounts`` (pages) int32."""
+        ``v_scale`` (layers, pages, KV heads) float32, positive and at most 2^121,
+        ``tables`` (slots, pages per slot), ``lengths`` (slots) and ``refcounts``
+        (pages) int32."""
         self = cls.__new__(cls)
         self._bind(k, v, k_scale, v_scale, tables, lengths, refcounts)
         return self

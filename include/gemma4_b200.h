@@ -336,7 +336,7 @@ int g4_prep_bwd(const g4_prep_args* args, void* stream);
  * [kv head][token][head_dim] codes of 8 bits (G4_KV8_E4M3 or G4_KV8_INT8).  A
  * block is one page of one KV head; it has one fp32 scale in k_scale / v_scale
  * [page][kv head], and its values are code * scale.  Codes are finite and scales
- * positive and finite; g4_kv8_append writes powers of two.  tables
+ * positive, at most 2^121; g4_kv8_append writes powers of two.  tables
  * [slot][pages_per_slot] lists a sequence's pages in order (-1: none).
  *
  * A call serves `batch` rows.  Row b uses table row slots[b] (b itself when slots
@@ -401,7 +401,8 @@ typedef struct g4_kv8_args {
  * is the least power of two 2^e with max|x| <= 448 * 2^e (e4m3) or 127 * 2^e
  * (int8) over its finite values; when tokens join a page that holds earlier ones
  * it only grows, and the earlier codes are requantised.  Infinities saturate, NaN
- * becomes 0.  Slots must be distinct: a slot listed again is left out (status).
+ * becomes 0, and every value is finite in bf16 (the largest bf16 values in e4m3, above
+ * 248 * 2^120, become 240 * 2^120).  Slots must be distinct: a slot listed again is left out (status).
  */
 int g4_kv8_append(const g4_kv8_args* args, void* stream);
 /* K and V of the rows' positions as bf16; zeros past a row's end and where the

@@ -9,16 +9,20 @@ from __future__ import annotations
 
 import numpy as np
 
-MIN_EXP, MAX_EXP = -100, 122
+MIN_EXP = -100
+# the largest exponent, and the largest code there: code * scale stays below 2^128
+MAX_EXP = {"e4m3": 120, "int8": 121}
+TOP_CODE = {"e4m3": 240.0, "int8": 127.0}
 EXHAUSTED, ROW_FULL, BAD_INDEX = 1, 2, 4
 
 
-def to_grid(x: np.ndarray, fmt: str) -> np.ndarray:
-    """Nearest code (ties to even), saturating; NaN becomes 0."""
+def to_grid(x: np.ndarray, fmt: str, exp: int = 0) -> np.ndarray:
+    """Nearest code (ties to even), saturating (under the scale 2^exp); NaN becomes 0."""
     x = np.where(np.isnan(x), 0.0, x)
     if fmt == "int8":
         return np.clip(np.rint(np.clip(x, -1e6, 1e6)), -127, 127)
-    x = np.clip(x, -448.0, 448.0)
+    top = TOP_CODE[fmt] if exp == MAX_EXP[fmt] else 448.0
+    x = np.clip(x, -top, top)
     _, e = np.frexp(x)  # |x| in [2^(e-1), 2^e)
     step = np.exp2(np.maximum(e - 1, -6) - 3.0)
     return np.rint(x / step) * step
@@ -30,7 +34,7 @@ def block_exponent(x: np.ndarray, fmt: str) -> int:
     finite = np.abs(x[np.isfinite(x)])
     largest = finite.max() if finite.size else 0.0
     e = MIN_EXP
-    while e < MAX_EXP and largest > top * 2.0 ** e:
+    while e < MAX_EXP[fmt] and largest > top * 2.0 ** e:
         e += 1
     return e
 
@@ -82,12 +86,14 @@ class PagedCache:
                         if a > first:
                             old = scales[layer, page, h]
                             m, oe = np.frexp(old)
-                            e = max(e, min(max(int(oe) - (m == 0.5), MIN_EXP), MAX_EXP))
+                            e = max(e, min(max(int(oe) - (m == 0.5), MIN_EXP),
+                                           MAX_EXP[self.fmt]))
                             held = codes[layer, page, h, :a - first]
                             if old != 2.0 ** e:
                                 codes[layer, page, h, :a - first] = to_grid(
-                                    held * old / 2.0 ** e, self.fmt)
-                        codes[layer, page, h, a - first:z - first] = to_grid(x / 2.0 ** e, self.fmt)
+                                    held * old / 2.0 ** e, self.fmt, e)
+                        codes[layer, page, h, a - first:z - first] = to_grid(
+                            x / 2.0 ** e, self.fmt, e)
                         scales[layer, page, h] = 2.0 ** e
 
     def read(self, layer, slots, starts, ends, max_tokens):

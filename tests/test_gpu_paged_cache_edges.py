@@ -13,7 +13,7 @@ if not torch.cuda.is_available():  # pragma: no cover - CPU containers
 
 from gemma4_fa4_kernels_b200 import PagedKVCache8, _lib  # noqa: E402
 from gemma4_fa4_kernels_b200.paged_cache import DIRECT_COLUMNS  # noqa: E402
-from test_gpu_paged_cache import Pair, bf16, check_attention, i32  # noqa: E402
+from test_gpu_paged_cache import Pair, bf16, check_attention, f64, i32  # noqa: E402
 
 BAD = _lib.G4_PAGES_BAD_INDEX
 
@@ -176,6 +176,59 @@ def test_rows_that_ask_for_more_than_31_bits_of_pages_together():
         cache.check()
     del tables, cache
     torch.cuda.empty_cache()
+
+
+# ------------------------------------------------------------------------------------
+# the largest values
+# ------------------------------------------------------------------------------------
+LARGEST = float(torch.finfo(torch.bfloat16).max)
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+def test_the_largest_values_stay_finite(fmt):
+    """Up to the largest BF16 value: codes and scales as the oracle's, read back finite
+    and off by at most 2^-4 of the value (e4m3) or half a step (int8)."""
+    rng = np.random.default_rng(60)
+    p = Pair(fmt, pages=12, slots=6, per_slot=4, page=16, d=256, heads=2)
+    x = LARGEST * rng.uniform(-1, 1, (5, 20, 2, 256))
+    x[0, 0, :, 0], x[1, 17, :, 3] = LARGEST, -LARGEST
+    x[2] *= 0.875                                 # up to 448 * 2^119
+    x[2, 5, :, 9] = 448 * 2.0 ** 119
+    x[3, 1, :, 7], x[3, 2, :, 8], x[3, 3, :, 9] = LARGEST, np.inf, np.nan
+    x[4], x[4, 4] = 1e-3 * x[4] / LARGEST, LARGEST  # ordinary ones under the largest scale
+    k, hk = bf16(x)
+    starts, ends = p.extend(list(range(5)), [20] * 5)
+    p.append(0, (k, hk), (-k, -hk), list(range(5)), starts, ends)
+    p.same()
+    p.fill(list(range(5)), [1] * 5, rng, magnitude=1e30)  # joins their pages
+    p.same()
+    got, _ = p.dev.read(0, i32(range(5)), i32(starts), i32(ends), 20)
+    got = f64(got)
+    assert np.isfinite(got).all()
+    ok = np.isfinite(hk) & (np.abs(hk) >= 2.0 ** 120)
+    err = np.abs(got - hk)[ok] / np.abs(hk)[ok]
+    if fmt == "e4m3":
+        assert err.max() <= 2.0 ** -4
+    else:
+        assert np.abs(got - hk)[ok].max() <= 2.0 ** 120
+    assert (np.abs(got[~np.isfinite(hk)]) <= LARGEST).all()
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("tokens", [1, 3, 9])
+def test_attention_over_the_largest_values(fmt, tokens):
+    """Decode and both wide shapes; V up to the largest BF16 value."""
+    rng = np.random.default_rng(61)
+    n = 150
+    p = Pair(fmt, heads=1, d=512, page=16, pages=12, slots=1, per_slot=10)
+    starts, ends = p.extend([0], [n])
+    k = rng.standard_normal((1, n, 1, 512))
+    v = LARGEST * rng.uniform(-1, 1, (1, n, 1, 512))
+    v[0, :, 0, 5] = LARGEST
+    p.append(0, k, v, [0], starts, ends)
+    q = 0.1 * rng.standard_normal((1, tokens, 8, 512))
+    got = check_attention(p, 0, q, [0], [n - tokens], [n])
+    assert np.isfinite(got).all()
 
 
 # ------------------------------------------------------------------------------------
