@@ -62,6 +62,12 @@ MAX_ROWS = 1024
 #   d256, window 1024    64 columns  32 / 36,   48 / 52    128 columns   34 / 36,   75 / 52
 DIRECT_COLUMNS = {512: 256, 256: 64}
 
+# Most bytes of that BF16 copy at once.  It is sized by the bound on the rows' keys, which
+# may be a whole slot, and the forward's own scratch grows with it: calls of more rows run
+# by groups of rows, one copy after another.  64 rows of 40 tokens behind 3000 keys, d512,
+# slots of 32768 tokens (us, GB at most): in one 1708, 41; with 9 GiB 1775, 21; 4 GiB 1902, 9.
+CHUNK_COPY_BYTES = 9 << 30
+
 
 def _layout(*shape) -> tuple:
     """(shape, strides) of a contiguous tensor."""
@@ -387,6 +393,25 @@ class PagedKVCache8:
             raise ValueError("q must be 16-byte aligned")
         window, max_k = a.window, a.max_seqlen_k
         keys = tokens + (min(max_k, window) if window else max_k) - 1  # most a row can see
+        rows = max(1, CHUNK_COPY_BYTES // (4 * keys * self.num_kv_heads * d))
+        if batch <= rows:
+            return self._chunk_rows(a, layer, q, out, slots, keys)
+        lse = self._new(_layout(batch, heads, tokens), torch.float32)
+        if slots is None:
+            slots = torch.arange(batch, dtype=torch.int32, device=self.device)
+        starts, ends = a.starts, a.ends
+        rows = -(-batch // -(-batch // rows))  # groups of about one size
+        for lo in range(0, batch, rows):
+            hi = min(lo + rows, batch)
+            a.batch, a.o = hi - lo, out[lo:hi].data_ptr()
+            a.slots = slots[lo:hi].data_ptr()
+            a.starts, a.ends = starts + 4 * lo, ends + 4 * lo
+            a.lse_stride[1] = (hi - lo) * tokens
+            lse[lo:hi] = self._chunk_rows(a, layer, q[lo:hi], out[lo:hi], slots[lo:hi], keys)
+        return lse
+
+    def _chunk_rows(self, a, layer, q, out, slots, keys):
+        batch, tokens, heads, d = q.shape
         total = batch * tokens
         lib = _lib.load()
         plan = torch.empty(5 * batch + 2, dtype=torch.int32, device=self.device)
@@ -401,7 +426,7 @@ class PagedKVCache8:
         self._read(self._read_block(layer, batch, keys), batch, slots, first, last, k, v, cu_k,
                    a.holes)
         with torch.cuda.device(self.device):
-            _, lse = ops.attn_fwd(q.reshape(total, heads, d), k, v, window=window,
+            _, lse = ops.attn_fwd(q.reshape(total, heads, d), k, v, window=a.window,
                                   cu_seqlens_q=cu_q, cu_seqlens_k=cu_k, max_seqlen_q=tokens,
                                   max_seqlen_k=keys, out=out.view(total, heads, d))
         a.q, a.lse = q.data_ptr(), lse.data_ptr()

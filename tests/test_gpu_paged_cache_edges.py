@@ -11,7 +11,7 @@ pytestmark = pytest.mark.gpu
 if not torch.cuda.is_available():  # pragma: no cover - CPU containers
     pytest.skip("needs a CUDA device", allow_module_level=True)
 
-from gemma4_fa4_kernels_b200 import PagedKVCache8, _lib  # noqa: E402
+from gemma4_fa4_kernels_b200 import PagedKVCache8, _lib, paged_cache  # noqa: E402
 from gemma4_fa4_kernels_b200.paged_cache import DIRECT_COLUMNS  # noqa: E402
 from test_gpu_paged_cache import Pair, bf16, check_attention, f64, i32  # noqa: E402
 
@@ -229,6 +229,50 @@ def test_attention_over_the_largest_values(fmt, tokens):
     q = 0.1 * rng.standard_normal((1, tokens, 8, 512))
     got = check_attention(p, 0, q, [0], [n - tokens], [n])
     assert np.isfinite(got).all()
+
+
+# ------------------------------------------------------------------------------------
+# memory
+# ------------------------------------------------------------------------------------
+@pytest.mark.parametrize("most", [None, 1 << 30])
+def test_the_copy_of_a_chunk_is_bounded_by_memory_not_by_rows(most, monkeypatch):
+    """64 rows of 40 tokens in slots of 32768 tokens: the bound alone would make the copy
+    of their keys 17 GB, and the forward's scratch 22."""
+    if most:
+        monkeypatch.setattr(paged_cache, "CHUNK_COPY_BYTES", most)
+    rng = np.random.default_rng(63)
+    rows, tokens = 64, 40
+    cache = PagedKVCache8(1, 64 * 4, 4, 512, max_slots=rows + 1, pages_per_slot=512, page_size=64)
+    lens = i32(rng.integers(tokens, 200, rows))
+    slots = i32(rng.permutation(rows))
+    starts, ends = cache.extend(slots, lens)
+    k, _ = bf16(rng.standard_normal((rows, 200, 4, 512)))
+    cache.append(0, k, -k, slots, starts, ends)
+    q, _ = bf16(0.2 * rng.standard_normal((rows, tokens, 32, 512)))
+    tight, tight_lse = cache.attention(0, q, slots, ends - tokens, ends, max_seqlen_k=200)
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    out, lse = cache.attention(0, q, slots, ends - tokens, ends)
+    torch.cuda.synchronize()
+    # the forward's scratch is about 1.4 times the copy
+    assert torch.cuda.max_memory_allocated() - before < 2.5 * paged_cache.CHUNK_COPY_BYTES
+    assert out.shape == tight.shape and lse.shape == tight_lse.shape
+    # another bound may run another kernel of the packed forward: P's 8 bits at most
+    assert (out - tight).abs().max() <= 2.0 ** -6 * tight.abs().max()
+    assert (lse - tight_lse).abs().max() <= 1e-4
+    every = cache.attention(0, q, None, *_by_slot(slots, ends - tokens, ends))
+    order = slots.long().argsort()
+    want = cache.attention(0, q, i32(range(rows)), (ends - tokens)[order], ends[order])
+    assert torch.equal(every[0], want[0]) and torch.equal(every[1], want[1])
+    cache.check()
+    torch.cuda.empty_cache()
+
+
+def _by_slot(slots, starts, ends):
+    order = slots.long().argsort()
+    return starts[order], ends[order]
 
 
 # ------------------------------------------------------------------------------------
