@@ -368,7 +368,9 @@ class PagedKVCache8:
         if max_k < 1:
             raise ValueError("max_seqlen_k must be positive")
         a = self._block(layer, batch, tokens)
-        a.num_q_heads, a.window, a.max_seqlen_k = heads, int(window), min(max_k, self.capacity)
+        # (no position reaches the capacity: a window beyond it is the same, and fits 31 bits)
+        a.num_q_heads, a.window = heads, min(int(window), self.capacity)
+        a.max_seqlen_k = min(max_k, self.capacity)
         a.q_stride[:] = _strides(q)
         a.o_stride[:] = (heads * tokens * d, heads * d, d)
         if any(s <= 0 or s % 8 for s in a.q_stride):
@@ -472,7 +474,7 @@ class PagedKVCache8:
         through a sliding window of ``window``; lengths stay."""
         if window < 1:
             raise ValueError("window must be positive")
-        self._free(slots, int(window))
+        self._free(slots, min(int(window), self.capacity))
 
     def _free(self, slots, window) -> None:
         batch = self._page_rows(slots, "slots")

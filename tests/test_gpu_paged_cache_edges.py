@@ -232,6 +232,27 @@ def test_attention_over_the_largest_values(fmt, tokens):
 
 
 # ------------------------------------------------------------------------------------
+# the largest windows
+# ------------------------------------------------------------------------------------
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 31, 2 ** 32, 2 ** 32 + 5])
+def test_windows_past_31_bits_reach_every_key(window):
+    rng = np.random.default_rng(62)
+    p = Pair("int8", heads=2, d=256, page=16, pages=30, slots=2, per_slot=12)
+    p.fill([0, 1], [150, 40], rng)
+    for tokens in (1, 9, 40):
+        q = 0.3 * rng.standard_normal((2, tokens, 4, 256))
+        at = [0, 1], [150 - tokens, 40 - tokens], [150, 40]
+        dq, _ = bf16(q)
+        want = p.dev.attention(0, dq, *map(i32, at))
+        got = p.dev.attention(0, dq, *map(i32, at), window=window)
+        # another mask may run another kernel of the packed forward: P's 8 bits at most
+        assert (got[0] - want[0]).abs().max() <= 2.0 ** -6 * want[0].abs().max()
+        assert (got[1] - want[1]).abs().max() <= 1e-4
+    p.dev.trim(i32([0, 1]), window)
+    p.same()
+
+
+# ------------------------------------------------------------------------------------
 # memory
 # ------------------------------------------------------------------------------------
 @pytest.mark.parametrize("most", [None, 1 << 30])
