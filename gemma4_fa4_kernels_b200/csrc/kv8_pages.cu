@@ -7,7 +7,9 @@
 // the lowest free ids in order of the call's rows, so results never depend on
 // timing.  Whole pages are shared between forks; the page a sequence still writes
 // to is its own (fork copies a partly filled last page), so an append never touches
-// another sequence's tokens.
+// another sequence's tokens.  A length may be lowered from outside (rejected drafts):
+// the pages behind it stay the slot's; extend fills them before it takes new ones, free
+// gives them back.
 //
 // Bound: the page copies are HBM copies; the rest is latency: one CTA scans the
 // refcounts (coalesced, one scan), then every table entry is one independent load
@@ -86,6 +88,8 @@ __device__ __forceinline__ int pages_of(int tokens, int shift) {
   return (tokens + (1 << shift) - 1) >> shift;
 }
 
+constexpr int kAhead = 4;  // table entries of a thread in flight
+
 __device__ __forceinline__ void raise(int* status, int bit) { atomicOr(status, bit); }
 
 // One unit of a page copy: 16 KB of codes of one layer's K or V (and, in the first,
@@ -125,6 +129,11 @@ __device__ __forceinline__ int64_t units_per_half(const Kv8PagesParams& p) {
 
 }  // namespace
 
+// Tables that list a page; 0 for an entry without one.
+__device__ __forceinline__ int page_refs(const Kv8PagesParams& p, int page) {
+  return page >= 0 && page < p.num_pages ? p.refcounts[page] : 0;
+}
+
 // Rows b in order: slot a[b] grows by counts[b] tokens.  starts/ends: the new
 // tokens' positions; a row that is not served gets start = end.
 __global__ void __launch_bounds__(kPlanThreads) pages_extend_kernel(const Kv8PagesParams p) {
@@ -134,7 +143,7 @@ __global__ void __launch_bounds__(kPlanThreads) pages_extend_kernel(const Kv8Pag
   __shared__ int have[kKv8MaxBatch];       // pages the row has; -1 not served
   pdl_enter();
   const int b = threadIdx.x;
-  int slot = -1, count = 0, len = 0, need = 0;
+  int slot = -1, count = 0, len = 0, need = 0, old = 0;  // old: pages the row has
   if (b < p.batch) {
     slot = p.a[b];
     count = p.counts[b];
@@ -153,7 +162,33 @@ __global__ void __launch_bounds__(kPlanThreads) pages_extend_kernel(const Kv8Pag
       ok = false;
       raise(p.status, kKv8RowFull);
     } else {
-      need = pages_of(len + count, p.page_shift) - pages_of(len, p.page_shift);
+      const int* row = p.tables + static_cast<int64_t>(slot) * p.pages_per_slot;
+      const int want = pages_of(len + count, p.page_shift);
+      old = pages_of(len, p.page_shift);
+      // The pages that the new tokens fill: the partly filled last one and, where the length
+      // was lowered, those listed behind it, up to the first entry without a page.  (The
+      // first step ends the search for a slot whose length was not.)
+      const int begin = old;
+      bool more = count > 0;
+      for (int j0 = begin - ((len & (p.page - 1)) != 0); more && j0 < want; j0 += kAhead) {
+        int page[kAhead], refs[kAhead];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) page[i] = j0 + i < want ? row[j0 + i] : -1;
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) refs[i] = page_refs(p, page[i]);
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+          if (!more) continue;
+          if (refs[i] > 1) ok = false;  // another sequence's page too
+          if (j0 + i >= begin) {
+            more = refs[i] == 1;
+            old += more;
+          }
+          more = more && ok;
+        }
+      }
+      need = ok ? want - old : 0;
+      if (!ok) raise(p.status, kKv8BadIndex);
     }
   }
   int total;
@@ -178,7 +213,7 @@ __global__ void __launch_bounds__(kPlanThreads) pages_extend_kernel(const Kv8Pag
   }
   if (b < p.batch) {
     first[b] = inc - need;
-    have[b] = ok ? pages_of(len, p.page_shift) : -1;
+    have[b] = ok ? old : -1;
     if (b == p.batch - 1) first[p.batch] = total;
   }
   __syncthreads();
@@ -221,7 +256,7 @@ __global__ void __launch_bounds__(kPlanThreads) pages_fork_plan_kernel(const Kv8
   bool ok = b < B && parent >= 0 && parent < p.num_slots && child >= 0 && child < p.num_slots;
   if (ok) {
     len = p.lengths[parent];
-    old = p.lengths[child];
+    old = p.lengths[child] != 0 || p.tables[static_cast<int64_t>(child) * p.pages_per_slot] >= 0;
   }
   __syncthreads();
   if (ok)
@@ -295,24 +330,38 @@ __global__ void __launch_bounds__(256) pages_fork_apply_kernel(const Kv8PagesPar
   }
 }
 
-// Row b: slot a[b] gives its pages back.  window 0: all of them, the row is empty
-// afterwards; window W: the leading pages that neither the next token at position
+// Row b: slot a[b] gives its pages back.  window 0: all that its table lists, the row is
+// empty afterwards; window W: the leading pages that neither the next token at position
 // `length` nor any later one sees (keys > position - W); the row keeps its length.
 // An entry is taken by an atomic exchange, so a slot listed twice frees once.
-__global__ void __launch_bounds__(128) pages_free_kernel(const Kv8PagesParams p) {
+constexpr int kFreeThreads = 256;
+__global__ void __launch_bounds__(kFreeThreads) pages_free_kernel(const Kv8PagesParams p) {
   pdl_enter();
   const int slot = p.a[blockIdx.x];
   if (slot < 0 || slot >= p.num_slots) {
     if (threadIdx.x == 0) raise(p.status, kKv8BadIndex);
     return;
   }
-  const int len = p.lengths[slot];
-  int upto = min(p.pages_per_slot, pages_of(max(len, 0), p.page_shift));
-  if (p.window > 0) upto = min(upto, max(0, len - p.window + 1) >> p.page_shift);
+  int upto = p.pages_per_slot;
+  if (p.window > 0) {
+    const int len = p.lengths[slot];
+    upto = min(min(upto, pages_of(max(len, 0), p.page_shift)),
+               max(0, len - p.window + 1) >> p.page_shift);
+  }
   int* row = p.tables + static_cast<int64_t>(slot) * p.pages_per_slot;
-  for (int j = threadIdx.x; j < upto; j += blockDim.x) {
-    const int page = atomicExch(&row[j], -1);
-    if (page >= 0 && page < p.num_pages) atomicSub(&p.refcounts[page], 1);
+  for (int j0 = threadIdx.x; j0 < upto; j0 += kAhead * kFreeThreads) {
+    int page[kAhead];
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      const int j = j0 + i * kFreeThreads;
+      page[i] = j < upto ? row[j] : -1;
+    }
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+      if (page[i] == -1) continue;
+      page[i] = atomicExch(&row[j0 + i * kFreeThreads], -1);
+      if (page[i] >= 0 && page[i] < p.num_pages) atomicSub(&p.refcounts[page[i]], 1);
+    }
   }
   __syncthreads();
   if (threadIdx.x == 0 && p.window == 0) p.lengths[slot] = 0;
@@ -413,7 +462,7 @@ int launch_pages_fork_apply(const Kv8PagesParams& p, int ctas, cudaStream_t st) 
 }
 int launch_pages_free(const Kv8PagesParams& p, cudaStream_t st) {
   return static_cast<int>(
-      launch_chained(pages_free_kernel, dim3(p.batch), dim3(128), 0, st, p));
+      launch_chained(pages_free_kernel, dim3(p.batch), dim3(kFreeThreads), 0, st, p));
 }
 int launch_pages_compact_plan(const Kv8PagesParams& p, cudaStream_t st) {
   return static_cast<int>(

@@ -38,6 +38,10 @@ current stream of the cache's device and do not wait for it, except ``check`` an
 for prompt chunks whose scratch exceeds the forward's budget, ``attention`` (as the
 packed forward does; such a call cannot be captured).  The cache's tensors are its own
 for its life: their contents may be changed from outside, they are not to be replaced.
+
+Rejected drafts are taken back by lowering their slots' ``lengths`` on the device
+(``cache.lengths[slots] = ends - rejected``): the pages behind a length stay the slot's,
+:meth:`extend` fills them before it takes new ones and :meth:`free` gives them back.
 """
 
 from __future__ import annotations
@@ -442,8 +446,8 @@ class PagedKVCache8:
         """Reserve pages for ``counts`` (int32 per row, or one int) more tokens of each
         slot and advance its length.  Returns ``(starts, ends)``, the new tokens'
         positions; a row that does not fit (its table is full, the pool has too few
-        pages left by the rows before it, its slot is bad or listed before) is left as
-        it was with start = end."""
+        pages left by the rows before it, its slot is bad or listed before, or its new
+        tokens would go into a page that it shares) is left as it was with start = end."""
         batch = self._page_rows(slots, "slots")
         if isinstance(counts, int):
             counts = torch.full((batch,), counts, dtype=torch.int32, device=self.device)
@@ -457,7 +461,7 @@ class PagedKVCache8:
         return starts, ends
 
     def fork(self, parents: torch.Tensor, children: torch.Tensor) -> None:
-        """Make each child (an empty slot) a copy of its parent: whole pages are
+        """Make each child (an empty slot without pages) a copy of its parent: whole pages are
         shared, a partly filled last page is copied in every layer."""
         batch = self._page_rows(parents, "parents")
         self._ints(children, batch, "children")

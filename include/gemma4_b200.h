@@ -473,9 +473,12 @@ typedef struct g4_pages_args {
 } g4_pages_args;
 
 size_t g4_pages_workspace_bytes(const g4_pages_args* args);
-/* Reserve pages for counts[b] more tokens of each slot and advance its length. */
+/* Reserve pages for counts[b] more tokens of each slot and advance its length.  A
+ * length may be lowered between calls: the pages behind it stay the slot's and are
+ * used first, g4_pages_free gives them back.  A slot whose new tokens would go into a
+ * page that another table lists is not served (G4_PAGES_BAD_INDEX). */
 int g4_pages_extend(const g4_pages_args* args, void* stream);
-/* Make each child (an empty slot) a copy of its parent: whole pages are shared, a
+/* Make each child (an empty slot without pages) a copy of its parent: whole pages are shared, a
  * partly filled last page is copied. */
 int g4_pages_fork(const g4_pages_args* args, void* stream);
 int g4_pages_free(const g4_pages_args* args, void* stream);

@@ -148,6 +148,11 @@ class PagedCache:
     def _slot(self, s):
         return 0 <= s < len(self.lengths)
 
+    def _refs(self, s, i):
+        """Tables that list slot s's i-th page; 0 where it has none."""
+        p = self.tables[s, i]
+        return self.refcounts[p] if 0 <= p < len(self.refcounts) else 0
+
     def extend(self, slots, counts):
         starts, ends = np.zeros(len(slots), int), np.zeros(len(slots), int)
         free = [p for p in range(len(self.refcounts)) if self.refcounts[p] == 0]
@@ -164,7 +169,16 @@ class PagedCache:
             if new > self.tables.shape[1] * self.page:
                 self.status |= ROW_FULL
                 continue
+            # pages behind a length that was lowered are used again
             have, want = -(-self.lengths[s] // self.page), -(-new // self.page)
+            if self.lengths[s] % self.page and n and self._refs(s, have - 1) > 1:
+                self.status |= BAD_INDEX
+                continue
+            while have < want and self._refs(s, have) == 1:
+                have += 1
+            if have < want and self._refs(s, have) > 1:
+                self.status |= BAD_INDEX
+                continue
             if want - have > len(free):
                 self.status |= EXHAUSTED
                 continue
@@ -185,7 +199,7 @@ class PagedCache:
         wanted = 0
         for b, (s, c) in enumerate(zip(parents, children)):
             if (not self._slot(s) or not self._slot(c) or c in list(children[:b])
-                    or before[c] != 0):
+                    or before[c] != 0 or self.tables[c, 0] >= 0):
                 self.status |= BAD_INDEX
                 continue
             whole, part = divmod(int(before[s]), self.page)
@@ -209,9 +223,10 @@ class PagedCache:
             if not self._slot(s):
                 self.status |= BAD_INDEX
                 continue
-            upto = -(-self.lengths[s] // self.page)
+            upto = self.tables.shape[1]
             if window:
-                upto = min(upto, max(0, self.lengths[s] - window + 1) // self.page)
+                upto = min(-(-self.lengths[s] // self.page),
+                           max(0, self.lengths[s] - window + 1) // self.page)
             for j in range(upto):
                 if self.tables[s, j] >= 0:
                     self.refcounts[self.tables[s, j]] -= 1

@@ -179,6 +179,69 @@ def test_rows_that_ask_for_more_than_31_bits_of_pages_together():
 
 
 # ------------------------------------------------------------------------------------
+# lengths that were lowered from outside: rejected drafts
+# ------------------------------------------------------------------------------------
+def _lower(p, slots, lengths):
+    for s, n in zip(slots, lengths):
+        p.ref.lengths[s] = n
+        p.dev.lengths[s] = n
+
+
+def test_pages_behind_a_lowered_length_are_used_again_and_given_back():
+    rng = np.random.default_rng(50)
+    p = Pair("e4m3", pages=20, slots=5, per_slot=150, page=16)
+    p.fill([0, 1, 2], [30, 33, 16], rng)
+    for step in range(6):                       # five drafts a step, most of them rejected
+        starts, ends = p.fill([0, 1, 2], [5, 5, 5], rng)
+        q = 0.3 * rng.standard_normal((3, 5, 4, 256))
+        check_attention(p, 0, q, [0, 1, 2], starts, ends)
+        _lower(p, [0, 1, 2], [s + 1 + step % 3 for s in starts])
+        p.same()
+    assert int((p.ref.refcounts > 0).sum()) == sum(int((p.ref.tables[s] >= 0).sum()) for s in range(5))
+    _lower(p, [0, 2], [0, 17])                  # a whole prompt taken back
+    p.fill([0, 2], [100, 20], rng)
+    p.same()
+    _lower(p, [0], [3])
+    p.ref.free([0, 1, 0, 2])
+    p.dev.free(i32([0, 1, 0, 2]))
+    p.same()
+    assert not p.ref.refcounts.any()
+
+
+def test_many_pages_behind_a_lowered_length_are_given_back():
+    p = Pair("int8", heads=1, pages=420, slots=2, per_slot=400, page=16)
+    p.extend([0, 1], [6000, 100])
+    _lower(p, [0], [20])
+    p.ref.free([0, 0])
+    p.dev.free(i32([0, 0]))
+    p.same()
+    assert int(p.ref.refcounts.sum()) == 7
+
+
+def test_shared_pages_behind_a_lowered_length_are_not_written():
+    rng = np.random.default_rng(51)
+    p = Pair("e4m3", pages=20, slots=6, per_slot=8, page=16)
+    p.fill([0, 1], [48, 20], rng)
+    p.ref.fork([0], [2])
+    p.dev.fork(i32([0]), i32([2]))
+    before = f64(p.dev.read(0, i32([2]), i32([0]), i32([48]), 48)[0])
+    for n in (30, 16, 0):                       # inside a shared page, at the start of one
+        _lower(p, [0], [n])
+        starts, ends = p.extend([0, 1], [4, 4])
+        assert starts[0] == ends[0] and p.ref.status == BAD
+        _lower(p, [1], [20])
+        p.same()
+    assert np.array_equal(before, f64(p.dev.read(0, i32([2]), i32([0]), i32([48]), 48)[0]))
+    p.ref.fork([1], [0])                        # a child that still holds pages is not empty
+    p.dev.fork(i32([1]), i32([0]))
+    p.same()
+    p.ref.free([0])
+    p.dev.free(i32([0]))
+    p.fill([2, 1], [1, 1], rng)                 # the pages are the child's alone now
+    p.same()
+
+
+# ------------------------------------------------------------------------------------
 # the largest values
 # ------------------------------------------------------------------------------------
 LARGEST = float(torch.finfo(torch.bfloat16).max)
