@@ -372,7 +372,7 @@ int g4_kv8_attn(const g4_kv8_args* a, void* stream) {
     rc = launch_kv8_attn(a->head_dim, a->format == G4_KV8_INT8, p, w.ctas, st);
     if (rc) return launched(rc, "cache attention launch");
   }
-  if (!w.whole && w.ctas > 1) {  // one CTA sums its own parts
+  if (!w.whole) {
     LaunchScope ls(kKKv8Merge, st);
     return launched(launch_kv8_merge(a->head_dim, p, w.ctas, st), "cache attention merge launch");
   }

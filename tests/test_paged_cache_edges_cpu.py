@@ -18,6 +18,16 @@ def test_chunk_plan_wants_the_rows_of_missing_pages():
     assert rc == _lib.G4_ERR_INVALID and "holes" in _lib.last_error()
 
 
+def test_equal_runs_have_a_place_for_their_parts():
+    """Any call that is not one CTA per item needs the parts' workspace and their merge."""
+    lib = _lib.load()
+    size = lambda **o: lib.g4_kv8_attn_workspace_bytes(ctypes.byref(_kv8(**o)))  # noqa: E731
+    assert size(max_seqlen_k=64) == 256  # one CTA per item
+    for over in (dict(batch=200, num_slots=200, max_seqlen_k=1), dict(pages_per_slot=64, max_seqlen_k=4096)):
+        # two parts per run and CTA, of 8 columns of 512 floats
+        assert size(**over) > 148 * 6 * 2 * 8 * 512 * 4
+
+
 def test_the_end_of_a_chunk_wants_them_too():
     for over, code, needle in ((dict(), _lib.G4_ERR_INVALID, "holes"),
                                (dict(holes=0xd000, q=None), _lib.G4_ERR_INVALID, "q is required"),
