@@ -123,11 +123,12 @@ __global__ void __launch_bounds__(512) kv8_append_kernel(const Kv8StoreParams p)
                                               (u % kPerRow) * kChunk);
   }
   const int page = kv8_page(c, row.slot, page_pos);
-  // a slot listed twice: the first row writes it, later ones are left out (two
+  // a slot that two rows write to: the first one does, later ones are left out (two
   // CTAs would race on the page's scale)
   if (p.rows.slots) {
     int dup = 0;
-    for (int j = threadIdx.x; j < b; j += blockDim.x) dup |= p.rows.slots[j] == row.slot;
+    for (int j = threadIdx.x; j < b; j += blockDim.x)
+      dup |= p.rows.slots[j] == row.slot && p.rows.ends[j] > p.rows.starts[j];
     if (__syncthreads_or(dup)) {
       if (threadIdx.x == 0 && p.status) atomicOr(p.status, kKv8BadIndex);
       return;

@@ -29,7 +29,7 @@ row with ``ends[b] <= starts[b]`` asks for nothing, whatever its slot.  One that
 asks for a slot or positions out of range counts as empty; a row that
 :meth:`extend`, :meth:`fork` or :meth:`copy_pages` cannot serve is left as it was.
 Both raise a bit of ``status``, which :meth:`check` turns into an exception.
-Slots of one call must be distinct.
+Slots of one call must be distinct; :meth:`append` overlooks rows that ask for nothing.
 
 Head dims 256 and 512 (local and global layers), any number of query heads per KV
 head, softmax scale 1, the causal and sliding-window masks of the attention
@@ -111,7 +111,7 @@ class PagedKVCache8:
 
     @classmethod
     def from_tensors(cls, k, v, k_scale, v_scale, tables, lengths, refcounts) -> "PagedKVCache8":
-        """A cache over existing tensors (kept, not copied): codes ``k``, ``v``
+        """A cache over existing tensors (kept, not copied): finite codes ``k``, ``v``
         (layers, pages, KV heads, page_size, head_dim), scales ``k_scale``,
         ``v_scale`` (layers, pages, KV heads) float32, positive and at most 2^121,
         ``tables`` (slots, pages per slot), ``lengths`` (slots) and ``refcounts``

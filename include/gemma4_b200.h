@@ -402,7 +402,8 @@ typedef struct g4_kv8_args {
  * (int8) over its finite values; when tokens join a page that holds earlier ones
  * it only grows, and the earlier codes are requantised.  Infinities saturate, NaN
  * becomes 0, and every value is finite in bf16 (the largest bf16 values in e4m3, above
- * 248 * 2^120, become 240 * 2^120).  Slots must be distinct: a slot listed again is left out (status).
+ * 248 * 2^120, become 240 * 2^120).  Slots must be distinct: a row whose slot an
+ * earlier row writes to is left out (status).
  */
 int g4_kv8_append(const g4_kv8_args* args, void* stream);
 /* K and V of the rows' positions as bf16; zeros past a row's end and where the

@@ -70,7 +70,7 @@ class PagedCache:
             n = self._row(slot, starts[b], ends[b], k.shape[1])
             if not n:
                 continue
-            if slot in slots[:b]:
+            if any(slots[j] == slot and ends[j] > starts[j] for j in range(b)):
                 self.status |= BAD_INDEX
                 continue
             for first in range(starts[b] // self.page * self.page, starts[b] + n, self.page):

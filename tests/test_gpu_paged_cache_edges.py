@@ -131,6 +131,21 @@ def test_rows_beyond_the_bound_of_a_call_are_reported(tokens):
     p.dev.check()
 
 
+def test_rows_that_ask_for_nothing_may_repeat_a_slot():
+    """The padding of a batch, before and behind the rows that it lists again."""
+    rng = np.random.default_rng(45)
+    p = Pair("e4m3")
+    starts, ends = p.extend([0, 2], [20, 5])
+    k, v = rng.standard_normal((2, 5, 20, 2, 256))
+    p.append(0, k, v, [0, 0, 2, 0, 2], [0, starts[0], starts[1], 20, 3],
+             [0, ends[0], ends[1], 20, 1])
+    assert p.ref.status == 0 and p.ref.k[0, 0].any()
+    p.same()
+    p.append(0, v, k, [2, 0, 2, 0, 2], [0, 3, 1, 4, 3], [0, 9, 4, 5, 3])  # row 3 is a repeat
+    assert p.ref.status == BAD
+    p.same()
+
+
 # ------------------------------------------------------------------------------------
 # a pool that runs out
 # ------------------------------------------------------------------------------------
