@@ -203,6 +203,9 @@ class PagedCache:
                 self.status |= BAD_INDEX
                 continue
             whole, part = divmod(int(before[s]), self.page)
+            if part and self._page(s, int(before[s])) < 0:  # trimmed, then lowered
+                self.status |= BAD_INDEX
+                continue
             if part:
                 wanted += 1
                 if wanted > len(free):

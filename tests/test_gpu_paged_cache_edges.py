@@ -71,6 +71,30 @@ def test_a_chunk_over_trimmed_pages():
     p.same()
 
 
+def test_captured_chunks_see_the_pages_of_their_replay():
+    rng = np.random.default_rng(46)
+    p = Pair("e4m3", heads=2, d=256, page=16, pages=40, slots=2, per_slot=20)
+    p.fill([0, 1], [200, 90], rng)
+    q, _ = bf16(0.2 * rng.standard_normal((2, 40, 4, 256)))
+    args = (0, q, i32([0, 1]), i32([160, 55]), i32([200, 90]))
+    p.dev.attention(*args)
+    torch.cuda.synchronize()
+    graphs = [torch.cuda.CUDAGraph() for _ in range(2)]
+    outs = []
+    for g in graphs:
+        with torch.cuda.graph(g):
+            outs.append(p.dev.attention(*args))
+    for hole in (None, (0, 3), (1, 5), None):
+        p.dev.tables.copy_(i32(p.ref.tables))
+        if hole:
+            p.dev.tables[hole] = -1
+        want = p.dev.attention(*args)
+        for g in graphs:
+            g.replay()
+        for out in outs:
+            assert torch.equal(out[0], want[0]) and torch.equal(out[1], want[1])
+
+
 # ------------------------------------------------------------------------------------
 # rows out of range
 # ------------------------------------------------------------------------------------
@@ -254,6 +278,37 @@ def test_shared_pages_behind_a_lowered_length_are_not_written():
     p.dev.free(i32([0]))
     p.fill([2, 1], [1, 1], rng)                 # the pages are the child's alone now
     p.same()
+
+
+@pytest.mark.parametrize("seed", range(6))
+def test_random_page_traffic_with_lowered_lengths(seed):
+    rng = np.random.default_rng(900 + seed)
+    pages = int(rng.integers(8, 90))
+    p = Pair("int8", heads=1, pages=pages, slots=12, per_slot=9, page=16, seed=seed)
+    for _ in range(40):
+        act, n = rng.integers(0, 8), int(rng.integers(1, 8))
+        slots = [int(s) for s in rng.choice(14, n, replace=False) - 1]
+        if act <= 1:
+            p.fill(slots, [int(x) for x in rng.integers(0, 60, n)], rng)
+        elif act == 2:
+            p.extend(slots, [int(x) for x in rng.integers(-1, 90, n)])
+        elif act == 3:
+            kids = [int(x) for x in rng.choice(12, n, replace=False)]
+            p.ref.fork(slots, kids)
+            p.dev.fork(i32(slots), i32(kids))
+        elif act == 4:
+            window = int(rng.choice([0, 0, 20, 60]))
+            p.ref.free(slots, window)
+            p.dev.trim(i32(slots), window) if window else p.dev.free(i32(slots))
+        elif act == 5:
+            p.ref.compact()
+            p.dev.compact()
+        else:
+            live = [s for s in slots if 0 <= s < 12 and p.ref.lengths[s] > 0]
+            # (to nothing only where the first page is still listed: an empty slot is a child)
+            _lower(p, live, [int(rng.integers(p.ref.tables[s, 0] < 0, p.ref.lengths[s] + 1))
+                             for s in live])
+        p.same()
 
 
 # ------------------------------------------------------------------------------------
