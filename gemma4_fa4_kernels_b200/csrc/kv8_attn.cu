@@ -40,9 +40,9 @@
 // power of two per column so that its largest element lies in [2^13, 2^14), then
 // held in fp16: exact down to elements 2^27 below the largest.  s_v P is held in
 // fp16 relative to its running maximum, which may lag by 2^3, and shifted up by
-// 2^11: below 2^15, rounded by at most 2^-12 of itself, or, for weights more than
+// 2^11: below 2^15, rounded by at most 2^-11 of itself, or, for weights more than
 // 2^25 below the largest, by 2^-36 of the largest.  The output's rounding to bf16
-// is 2^-9 of it.
+// is at most 2^-8 of it.
 #include <algorithm>
 
 #include "g4_kernels.h"

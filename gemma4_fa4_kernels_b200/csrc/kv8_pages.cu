@@ -426,7 +426,10 @@ __global__ void __launch_bounds__(256) pages_compact_apply_kernel(const Kv8Pages
 
 // Pair i: page a[i] to page b[i], all layers, K and V and their scales.  A pair is
 // left out (status bit) when an id is out of range, when an earlier pair has the
-// same destination, or when its destination is any pair's source.
+// same destination, or when its destination is any pair's source.  Every CTA checks the
+// pairs that it copies against all of them, without a workspace or a second launch: the
+// checks grow with the square of the pairs.  Copies (us, with the floor of their bytes): 200
+// pages of 256 KB in ten layers 173 / 160, 4096 pages of 8 KB 46 / 10, 16384 of them 475 / 41.
 __global__ void __launch_bounds__(256) pages_copy_kernel(const Kv8PagesParams p) {
   pdl_enter();
   const int64_t units = units_per_half(p);

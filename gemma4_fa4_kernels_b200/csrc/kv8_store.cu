@@ -1,5 +1,5 @@
 // Writing to and reading from the 8-bit paged KV cache: append (quantise), read
-// back (dequantise), and the small kernels around a prompt chunk's attention.
+// back (dequantise), and the plan of a prompt chunk's attention.
 //
 // Append.  A block (page, KV head) has the scale 2^e with the least e such that
 // its largest finite magnitude is at most `top` * 2^e (448 for e4m3, 127 for

@@ -12,8 +12,8 @@
 // swizzle), which the MMA reads once: 4 bytes of shared-memory traffic per code, at
 // 128 bytes per clock 32 codes per clock and SM, against the SM's share of HBM of 23;
 // in practice the converters' issue slots and the waits between tiles.  Five drafted
-// tokens of 8 heads (40 columns) over 6 rows of 700 to 9001 int8 keys: 45 us with 14 us for
-// the merge behind it, 94 and 12 with three blocks of 8 columns per pass of mma.sync.
+// tokens of 8 heads (40 columns) over 6 rows of 700 to 9001 int8 keys: 50 us a call with its
+// merge (alone and cold 50 and 14), 95 with three blocks of 8 columns per pass of mma.sync.
 //
 // Warp roles: 8 softmax warps (two per 32 TMEM lanes, thread = key, half of the columns
 // each), one MMA warp, three pairs of converter warps.  The pairs take turns: each keeps
@@ -48,9 +48,9 @@ constexpr int kConvWarps = 2 * kFeeds;
 constexpr int kWideThreads = (kSoft + 1 + kConvWarps) * 32;
 // s_v P in fp16 relative to O's reference, whose s_v counts as the power of two above
 // it: a reference that may lag by 2^9 and a shift of 2^6 keep P below 2^15; its largest
-// is at least 2^5, so half a step is 2^-12 of a weight, or 2^-30 of the largest for
-// weights more than 2^19 below it.  Renewals, which cost as much as the rest of a tile,
-// stay rare.
+// is at least 2^5, so half a step is at most 2^-11 of a weight, or 2^-30 of the largest
+// for weights more than 2^19 below it.  Renewals, which cost as much as the rest of a tile,
+// stay rare.  A softmax weight below 2^-126 of the largest is zero before its s_v counts.
 constexpr float kWideShift = 6.f;
 constexpr float kWideStale = 9.f;
 constexpr float kStaleSum = 8.f;   // log2 by which the row sum's reference may lag

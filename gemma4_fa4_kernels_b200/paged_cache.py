@@ -60,7 +60,10 @@ MAX_ROWS = 1024
 
 # Up to this many (token, query head) columns per KV head and row, by head dim, the
 # queries read the codes directly; longer chunks of prompts run the tensor-core forward
-# over a BF16 copy of the keys they see.  Measured, us, direct against copy (1 and 4 rows):
+# over a BF16 copy of the keys they see, whose softmax weights are BF16 (error against 64
+# bits 0.0023 of the output's size, 0.0017 directly).  One bound for any number of rows:
+# with one row the direct kernels stay faster beyond it, with four they do not.  Measured,
+# us, direct against copy (1 and 4 rows):
 #   d512, 1500 keys     256 columns  38 / 65,   71 / 81    512 columns   46 / 67,  116 / 85
 #   d512, 17000 keys    256 columns 118 / 419, 374 / 587   512 columns  206 / 423, 712 / 595
 #   d256, window 1024    64 columns  32 / 36,   48 / 52    128 columns   34 / 36,   75 / 52

@@ -412,8 +412,9 @@ int g4_kv8_read(const g4_kv8_args* args, void* stream);
 /*
  * Attention of the rows' queries (softmax scale 1) over the keys 0 .. position of
  * their own sequence, cut by the window; the keys of missing pages are masked.
- * A query without a visible key, and padding, gets O = 0 and LSE = -inf.  Meant
- * for a few queries per row; g4_kv8_chunk_plan serves prompt chunks.
+ * A query without a visible key, and padding, gets O = 0 and LSE = -inf.  Softmax
+ * weights below 2^-126 of a query's largest may count as zero.  Meant for a few
+ * queries per row; g4_kv8_chunk_plan serves prompt chunks.
  */
 size_t g4_kv8_attn_workspace_bytes(const g4_kv8_args* args);
 int g4_kv8_attn(const g4_kv8_args* args, void* stream);
@@ -460,7 +461,8 @@ typedef struct g4_pages_args {
   int32_t head_dim;
   int32_t num_slots;
   int32_t pages_per_slot;
-  int32_t batch;         /* rows of this call, at most 1024 (copy: any number) */
+  int32_t batch;         /* rows of this call, at most 1024 (copy: any number, whose checks
+                            grow with its square) */
   const int32_t* first;  /* extend, free: slots; fork: parents; copy: source pages */
   const int32_t* second; /* fork: children; copy: destination pages */
   const int32_t* counts; /* extend: new tokens */
